@@ -347,6 +347,112 @@ int lv_kernel_attention(lv_ctx *ctx, float *out, const void *kcache, const void 
 int lv_kernel_attention_static(lv_ctx *ctx, float *out, const void *kcache, const void *vcache, const float *q,
                                uint32_t pos, uint32_t backlog, uint32_t heads, uint32_t rot, uint32_t batch);
 
+/* ---- a serving step over a paged cache (no counterpart in the reference, which holds one sequence a session) ---------------
+ *      Several sequences keep their keys and values in pages of one pool.  In every layer of a step a program turns queries and keys by
+ *      their positions (lv_kernel_rotate), writes the new rows (lv_kernel_paged_write) and lets the new tokens attend to all that their
+ *      sequences hold (lv_kernel_paged_attention); where tokens were drafted, lv_kernel_verify_drafts finds out how many of them stand.
+ *
+ *      All pointers below are device pointers of the context's device, structs are host memory and borrowed for the call.  Calls are
+ *      asynchronous on the context's stream (lv_ctx_stream), allocate nothing and keep nothing, so they can be captured into a graph; what
+ *      they read on the device (lengths, pages, ...) may change between replays.  A workspace is written before it is read; two calls that
+ *      can overlap, as two captured graphs can, each need one of their own.
+ *      Row strides (ld*) count elements.  The pool, workspaces and the rows of q, k, v, x and out (pointer and stride in bytes) are aligned to 16 bytes,
+ *      everything else to 4.  The calls leave the caller's current device as it was. */
+
+/* the stream all work of a context runs on (a hipStream_t, non-blocking), for callers that order other work with it or capture it */
+int lv_ctx_stream(const lv_ctx *ctx, void **stream);
+
+/* A pool of `pages` pages, each `page` tokens long; a page holds the rows of all kv heads.  Page p, head h is a block of bytes at
+ * data + (p * kv_heads + h) * (lv_paged_cache_bytes / pages / kv_heads):
+ *     keys: codes [page][..], scales [page][dim / 32]; values: codes, scales
+ * LV_F16, LV_BF16: 2 bytes an element, no scales.  LV_Q8_0: an int8 an element, LV_Q4_0: 16 bytes for 32 elements, byte j holding element j in
+ * its low nibble and j + 16 in its high one, minus 8; both with an fp16 scale for every 32 elements (the blocks of GGML files, codes and scales apart).
+ * A block is stored with the scale d = fp16(min(max|x| * (1 / 127), 515.5)) and codes rint(x * (1 / d)) in -127 .. 127 (LV_Q8_0), or with
+ * d = fp16(clamp(m * -0.125, -8188, 8188)), m the element furthest from 0 (the positive one of two), and codes in -8 .. 7 (LV_Q4_0); steps in fp32, ties to
+ * even; a scale of 0 is +0, and so are its codes.  No stored value is beyond 65504; a NaN is stored as 0. */
+typedef struct {
+    void *data;
+    uint32_t type;               /* LV_F16, LV_BF16, LV_Q8_0, LV_Q4_0 */
+    uint32_t kv_heads, dim;      /* dim: 32, 64, 128 or 256 */
+    uint32_t page;               /* tokens a page: a power of two from 16 to 1024 */
+    uint32_t pages;
+} lv_paged_cache;
+/* bytes the pool needs at `data` (which is not looked at) */
+int lv_paged_cache_bytes(const lv_paged_cache *cache, uint64_t *bytes);
+
+/* The new tokens of a step.  Rows starts[b] .. starts[b + 1] - 1 of a call's tensors belong to sequence b and are the last of its lens[b]
+ * tokens; a sequence may have none.  Position i of sequence b lies in page table[b * table_ld + i / page].  Rows from starts[seqs] on belong to nobody and
+ * are left as they were (a padded batch).  starts are non-decreasing and at most `tokens`.  A position whose page is not in 0 .. pages - 1, or beyond
+ * the table, is never touched: it is not written, not read back, and hidden from attention; so is a position before 0 (lens[b] less than the new
+ * tokens). */
+typedef struct {
+    uint32_t seqs;               /* at most 65535 */
+    uint32_t tokens;             /* rows of the tensors */
+    const uint32_t *starts;      /* seqs + 1 */
+    const uint32_t *lens;        /* seqs */
+    const uint32_t *table;
+    uint32_t table_ld;           /* pages a row of the table; table_ld * page at most 2^30 */
+} lv_paged_batch;
+
+/* rows of keys and values, [tokens][kv_heads][dim] of `type` (LV_F32, LV_F16, LV_BF16), to their pages.  No two sequences may write to one place: a
+ * page that sequences share is written by none of them. */
+int lv_kernel_paged_write(lv_ctx *ctx, const lv_paged_cache *cache, const lv_paged_batch *batch, const void *k, uint32_t ldk, const void *v,
+                          uint32_t ldv, uint32_t type);
+/* the same rows back: what is stored, rounded once to `type` */
+int lv_kernel_paged_read(lv_ctx *ctx, const lv_paged_cache *cache, const lv_paged_batch *batch, void *k, uint32_t ldk, void *v, uint32_t ldv,
+                         uint32_t type);
+
+typedef struct {
+    uint32_t heads;              /* a multiple of kv_heads: heads / kv_heads consecutive ones share a key head */
+    float scale;
+    uint32_t window;             /* a position sees the last `window` ones, itself included; 0: all */
+    uint32_t chunk;              /* as in lv_attn_spec: a position sees its own chunk of this many positions, up to itself; 0: everything up to itself */
+    const float *sinks;          /* null, or one logit a head that joins the softmax denominator */
+} lv_paged_attn_spec;
+/* out[row][head][dim] = sum_p softmax_p(scale q . k_p) v_p over the positions p that the row's token sees, q and out [tokens][heads][dim] of `type`
+ * (LV_F32: as exact as fp32; LV_F16, LV_BF16: products of 16-bit operands, softmax and sums in fp32).  A row that sees nothing is 0.  The rows
+ * of keys and values of the new tokens have to be in the cache.  `work`: lv_paged_attention_workspace bytes, null where that is 0. */
+int lv_paged_attention_workspace(lv_ctx *ctx, uint32_t type, const lv_paged_cache *cache, const lv_paged_batch *batch, const lv_paged_attn_spec *spec,
+                                 uint64_t *bytes);
+int lv_kernel_paged_attention(lv_ctx *ctx, void *out, uint32_t ldo, const void *q, uint32_t ldq, uint32_t type, const lv_paged_cache *cache,
+                              const lv_paged_batch *batch, const lv_paged_attn_spec *spec, void *work, uint64_t work_bytes);
+
+/* Rotary positions: pair i of a head, i = 0 .. rot_dims / 2 - 1, turns by position * rot_base^(-2 i / rot_dims); the other elements stay.  Pairs are
+ * neighbours (2 i, 2 i + 1), or with LV_ROTATE_HALVES (i, i + rot_dims / 2).  The first sections[0] pairs take their position from the first axis, the next
+ * sections[1] from the second, sections[2] from the third (time, height, width); all 0: one axis for all.  With LV_ROTATE_PER_AXIS the exponent starts
+ * anew in every section, i counted inside it and its own size in place of rot_dims / 2. */
+enum { LV_ROTATE_HALVES = 1, LV_ROTATE_PER_AXIS = 2 };
+typedef struct {
+    uint32_t rot_dims;           /* even, at most dim */
+    double rot_base;             /* above 0 */
+    uint32_t sections[3];        /* sum rot_dims / 2, or all 0 */
+    uint32_t flags;
+} lv_rotate_spec;
+/* out[row][head][dim] from x[row][head][dim], both of `type` (LV_F32, LV_F16, LV_BF16); out may be x (the same pointer and stride), and overlaps it in no other
+ * way.  positions: [axes][tokens], as many axes as the last section that is not 0.  dim: a multiple of 8, at most 512.  Angles are formed in double. */
+int lv_kernel_rotate(lv_ctx *ctx, void *out, uint32_t ldo, const void *x, uint32_t ldx, uint32_t type, const uint32_t *positions, uint32_t tokens,
+                     uint32_t heads, uint32_t dim, const lv_rotate_spec *spec);
+
+/* Which drafted tokens stand.  Of sequence b, draft i (0 <= i < counts[b]) with token x stands while uniforms[b][i] * draft[b][i][x] < target[b][i][x] and
+ * all before it stand.  The next token comes from the row r = number of those that stand: from max(0, target[b][r] - draft[b][r]) if draft r was
+ * refused, from target[b][r] if there was none; it is the first j whose running sum is more than uniforms[b][drafts] times the whole.  Where no weight is left,
+ * the draw is from target[b][r], and where that has none either, it is token 0.  Weights that are negative or NaN count as 0, a draft outside the vocabulary
+ * is refused.  draft null: the drafts were picked, not sampled; their probability is 1.  Products and sums in double. */
+typedef struct {
+    uint32_t seqs, drafts, vocab;    /* drafts: columns of `tokens`, 1 to 64 */
+    const float *target;             /* [seqs][drafts + 1][vocab] probabilities, ld_target floats a row */
+    uint32_t ld_target;
+    const float *draft;              /* null, or [seqs][drafts][vocab], ld_draft floats a row */
+    uint32_t ld_draft;
+    const uint32_t *tokens;          /* [seqs][drafts] */
+    const uint32_t *counts;          /* null (all of them), or drafts of each sequence, at most `drafts` (more count as `drafts`) */
+    const float *uniforms;           /* [seqs][drafts + 1], in 0 .. 1, 1 excluded */
+} lv_draft_batch;
+enum { LV_NO_TOKEN = 0xffffffffu };
+/* tokens: [seqs][drafts + 1], the drafts that stand, the next token, LV_NO_TOKEN behind it; accepted: [seqs], how many drafts stand */
+int lv_verify_drafts_workspace(lv_ctx *ctx, const lv_draft_batch *batch, uint64_t *bytes);
+int lv_kernel_verify_drafts(lv_ctx *ctx, uint32_t *tokens, uint32_t *accepted, const lv_draft_batch *batch, void *work, uint64_t work_bytes);
+
 #ifdef __cplusplus
 }
 #endif

@@ -23,6 +23,8 @@ LV_F32, LV_F16, LV_Q4_0, LV_Q8_0, LV_BF16 = 0, 1, 2, 8, 30
 ATTN_NORM_FULL, ATTN_KEYS_AS_VALUES, ATTN_SINK = 1, 2, 4
 ACT_SILU, ACT_RELU = 0, 1
 NORM_RMS, NORM_TANH = 0, 1
+ROTATE_HALVES, ROTATE_PER_AXIS = 1, 2
+NO_TOKEN = 0xFFFFFFFF
 PATH_AUTO, PATH_KERNELS, PATH_GRAPH, PATH_PERSISTENT = range(4)
 TRACE_NORM_IN, TRACE_POST_ATTN, TRACE_POST_ATTN_NORM, TRACE_FF, TRACE_OUT, TRACE_ATTN = range(6)
 
@@ -78,6 +80,31 @@ class BlockHParams(C.Structure):
     _fields_ = [("vocab", C.c_uint32), ("dim", C.c_uint32), ("layers", C.c_uint32), ("eps", C.c_float), ("norm", C.c_uint32), ("streams", C.c_uint32),
                 ("tied_head", C.c_uint32), ("embed_scale", C.c_float), ("bigram_buckets", C.c_uint32), ("bigram_prev", C.c_uint32), ("bigram_cur", C.c_uint32),
                 ("loop_start", C.c_uint32), ("loop_stop", C.c_uint32), ("loop_times", C.c_uint32)]
+
+
+class PagedCache(C.Structure):
+    """lv_paged_cache: a pool of pages; data is a device pointer"""
+    _fields_ = [("data", C.c_void_p), ("type", C.c_uint32), ("kv_heads", C.c_uint32), ("dim", C.c_uint32), ("page", C.c_uint32), ("pages", C.c_uint32)]
+
+
+class PagedBatch(C.Structure):
+    """lv_paged_batch: the new tokens of a step; starts, lens, table are device pointers"""
+    _fields_ = [("seqs", C.c_uint32), ("tokens", C.c_uint32), ("starts", C.c_void_p), ("lens", C.c_void_p), ("table", C.c_void_p), ("table_ld", C.c_uint32)]
+
+
+class PagedAttnSpec(C.Structure):
+    """lv_paged_attn_spec; sinks is a device pointer or None"""
+    _fields_ = [("heads", C.c_uint32), ("scale", C.c_float), ("window", C.c_uint32), ("chunk", C.c_uint32), ("sinks", C.c_void_p)]
+
+
+class RotateSpec(C.Structure):
+    _fields_ = [("rot_dims", C.c_uint32), ("rot_base", C.c_double), ("sections", C.c_uint32 * 3), ("flags", C.c_uint32)]
+
+
+class DraftBatch(C.Structure):
+    """lv_draft_batch; all but the sizes are device pointers, draft and counts may be None"""
+    _fields_ = [("seqs", C.c_uint32), ("drafts", C.c_uint32), ("vocab", C.c_uint32), ("target", C.c_void_p), ("ld_target", C.c_uint32), ("draft", C.c_void_p),
+                ("ld_draft", C.c_uint32), ("tokens", C.c_void_p), ("counts", C.c_void_p), ("uniforms", C.c_void_p)]
 
 
 class MkgConfig(C.Structure):
@@ -170,6 +197,15 @@ _HIP_SIGS = {
     "lv_kernel_kv_append": [_VP, _VP, _VP, _U32, _U32, _U32, _U32],
     "lv_kernel_attention": [_VP, _VP, _VP, _VP, _VP, _U32, _U32, _U32, _U32, _U32],
     "lv_kernel_attention_static": [_VP, _VP, _VP, _VP, _VP, _U32, _U32, _U32, _U32, _U32],
+    "lv_ctx_stream": [_VP, C.POINTER(_VP)],
+    "lv_paged_cache_bytes": [C.POINTER(PagedCache), C.POINTER(_U64)],
+    "lv_kernel_paged_write": [_VP, C.POINTER(PagedCache), C.POINTER(PagedBatch), _VP, _U32, _VP, _U32, _U32],
+    "lv_kernel_paged_read": [_VP, C.POINTER(PagedCache), C.POINTER(PagedBatch), _VP, _U32, _VP, _U32, _U32],
+    "lv_paged_attention_workspace": [_VP, _U32, C.POINTER(PagedCache), C.POINTER(PagedBatch), C.POINTER(PagedAttnSpec), C.POINTER(_U64)],
+    "lv_kernel_paged_attention": [_VP, _VP, _U32, _VP, _U32, _U32, C.POINTER(PagedCache), C.POINTER(PagedBatch), C.POINTER(PagedAttnSpec), _VP, _U64],
+    "lv_kernel_rotate": [_VP, _VP, _U32, _VP, _U32, _U32, _VP, _U32, _U32, _U32, C.POINTER(RotateSpec)],
+    "lv_verify_drafts_workspace": [_VP, C.POINTER(DraftBatch), C.POINTER(_U64)],
+    "lv_kernel_verify_drafts": [_VP, _VP, _VP, C.POINTER(DraftBatch), _VP, _U64],
 }
 
 
@@ -258,6 +294,45 @@ class Context:
 
     def matrix_free(self, m):
         check(self.lib.lv_matrix_destroy(m))
+
+    def stream(self):
+        """the stream this context's work runs on, as an integer"""
+        p = C.c_void_p()
+        check(self.lib.lv_ctx_stream(self.h, C.byref(p)))
+        return p.value
+
+    # a serving step over a paged cache; pointers and strides as in include/llava_hip.h
+    def rotate(self, out, ldo, x, ldx, type, positions, tokens, heads, dim, spec):
+        check(self.lib.lv_kernel_rotate(self.h, out, ldo, x, ldx, type, positions, tokens, heads, dim, spec))
+
+    def paged_write(self, cache, batch, k, ldk, v, ldv, type):
+        check(self.lib.lv_kernel_paged_write(self.h, cache, batch, k, ldk, v, ldv, type))
+
+    def paged_read(self, cache, batch, k, ldk, v, ldv, type):
+        check(self.lib.lv_kernel_paged_read(self.h, cache, batch, k, ldk, v, ldv, type))
+
+    def paged_attention_workspace(self, type, cache, batch, spec):
+        n = C.c_uint64()
+        check(self.lib.lv_paged_attention_workspace(self.h, type, cache, batch, spec, n))
+        return n.value
+
+    def paged_attention(self, out, ldo, q, ldq, type, cache, batch, spec, work=None, work_bytes=0):
+        check(self.lib.lv_kernel_paged_attention(self.h, out, ldo, q, ldq, type, cache, batch, spec, work, work_bytes))
+
+    def verify_drafts_workspace(self, batch):
+        n = C.c_uint64()
+        check(self.lib.lv_verify_drafts_workspace(self.h, batch, n))
+        return n.value
+
+    def verify_drafts(self, tokens, accepted, batch, work, work_bytes):
+        check(self.lib.lv_kernel_verify_drafts(self.h, tokens, accepted, batch, work, work_bytes))
+
+
+def paged_cache_bytes(cache):
+    """bytes a pool of pages needs"""
+    n = C.c_uint64()
+    check(hip().lv_paged_cache_bytes(cache, n))
+    return n.value
 
 
 # ----------------------------------------------------------------------------------------------------------

@@ -39,7 +39,7 @@ def hipcc():
     raise RuntimeError("hipcc not found: the HIP library cannot be built on this machine")
 
 
-HIP_UNITS = ("lv_api", "lv_block")    # translation units of libllava_hip.so, compiled side by side
+HIP_UNITS = ("lv_api", "lv_block", "lv_serve", "lv_paged")    # translation units of libllava_hip.so, compiled side by side
 
 
 def build_hip():

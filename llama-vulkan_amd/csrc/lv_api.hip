@@ -376,6 +376,17 @@ extern "C" int lv_ctx_info(const lv_ctx *c, char *name, size_t cap, uint32_t *cu
     return LV_OK;
 }
 
+extern "C" int lv_ctx_stream(const lv_ctx *c, void **stream)
+{
+    if (!c || !stream) return fail(LV_ERR_ARG, "lv_ctx_stream: null argument");
+    *stream = c->stream;
+    return LV_OK;
+}
+
+hipStream_t lv::ctx_stream(const lv_ctx *c) { return c->stream; }
+int lv::ctx_device(const lv_ctx *c) { return c->device; }
+uint32_t lv::ctx_units(const lv_ctx *c) { return (uint32_t)c->props.multiProcessorCount; }
+
 extern "C" int lv_ctx_sync(lv_ctx *c)
 {
     if (!c) return fail(LV_ERR_ARG, "lv_ctx_sync: ctx is null");

@@ -14,6 +14,11 @@ int fail(int code, const char *fmt, ...) __attribute__((format(printf, 2, 3)));
 // zero fill by a kernel on the stream (usable inside graph capture, unlike a memset node); bytes a multiple of 4
 int zero_async(void *p, uint64_t bytes, hipStream_t st);
 
+// a context's stream, device and compute units, for the entry points outside lv_api.hip
+hipStream_t ctx_stream(const lv_ctx *c);
+int ctx_device(const lv_ctx *c);
+uint32_t ctx_units(const lv_ctx *c);
+
 }  // namespace lv
 
 #define HIP_TRY(expr)                                                                                         \

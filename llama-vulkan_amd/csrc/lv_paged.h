@@ -1,0 +1,691 @@
+// lv_paged.h — attention of new tokens over the pages of their sequences (lv_kernel_paged_attention).
+//
+// A row is a new token and one of the heads that share a key head; scores are computed transposed, S^T = K Q^T, on
+// v_mfma_f32_16x16x32: a lane then holds scores of ONE row (column lane % 16), so maximum, rescaling and sum are per-lane numbers, and the registers of
+// S^T are the second operand of O^T = V^T P^T as they are (any order of the 32 keys of a product does, as long as both operands have the same).  V^T comes
+// from row-major values through ds_read_b64_tr_b16, which hands lane i of 16 the column i of 4 rows.
+//
+// Scores are in units of log2, 2^12 on top of the weights of fp16 products (a weight below 2^-14 of the largest would be an fp16 subnormal), which the sum has
+// as well.  Masked scores are -inf, the running maximum starts at a finite -1e30: a row that sees nothing ends with a sum of 0 and is written as 0.
+#pragma once
+
+#include "lv_common.h"
+#include "lv_device.h"
+#include "lv_paged_plan.h"
+
+namespace lv {
+
+typedef _Float16 pg_h8 __attribute__((ext_vector_type(8)));
+typedef _Float16 pg_h2 __attribute__((ext_vector_type(2)));
+typedef __bf16 pg_b8 __attribute__((ext_vector_type(8)));
+typedef float pg_f4 __attribute__((ext_vector_type(4)));
+typedef short pg_s4 __attribute__((ext_vector_type(4)));
+typedef short pg_s8 __attribute__((ext_vector_type(8)));
+
+enum { kPgF16 = 0, kPgBf16 = 1, kPgQ8 = 2, kPgQ4 = 3 };
+
+struct PagedAttnArgs {
+    PagedView c;
+    PagedDeal deal;
+    const uint32_t *starts, *lens, *table;
+    uint32_t table_ld;
+    const void *q;
+    void *out;
+    uint32_t ldq, ldo, type;
+    float scale;                // times log2 e
+    const float *sinks;
+    float *part, *part_ml;      // of cut items: [item][kv head][tile][dim], [item][kv head][tile][2]
+};
+
+// ---- which item ------------------------------------------------------------------------------------------------------------------
+struct PagedItem {
+    PagedSeq s;
+    uint32_t seq, tile, part, parts, run;
+    uint32_t first;                           // item of this tile's part 0
+    bool any;
+};
+
+__device__ __forceinline__ uint32_t wave_running_sum_u32(uint32_t v)
+{
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x111, 0xf, 0xf, true);      // row_shr 1, 2, 4, 8
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x112, 0xf, 0xf, true);
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x114, 0xf, 0xf, true);
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x118, 0xf, 0xf, true);
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x142, 0xa, 0xf, false);
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x143, 0xc, 0xf, false);
+    return v;
+}
+
+__device__ __forceinline__ PagedSeq paged_seq_of(const PagedAttnArgs &a, uint32_t b)
+{
+    return paged_seq(a.starts[b], a.starts[b + 1], a.lens[b], a.deal.tokens, a.deal.positions);
+}
+
+// steps of all tiles of all sequences: the same sum in every wave of both launches
+__device__ __forceinline__ float paged_all_steps(const PagedAttnArgs &a, int lane)
+{
+    float sum = 0.f;
+    for (uint32_t b0 = 0; b0 < a.deal.seqs; b0 += 64) {
+        float steps = 0.f;
+        if (b0 + lane < a.deal.seqs) {
+            const PagedSeq s = paged_seq_of(a, b0 + lane);
+            steps = (float)paged_tiles(a.deal, s) * (float)paged_steps(a.deal, s);
+        }
+        sum += wave_sum(steps);
+    }
+    return sum;
+}
+
+// The sequence that an item (BY_ROW false) or a row of the tensors (true; `sub`: which of the heads that share a key head) belongs to, found by each wave on its own.
+template <bool BY_ROW> __device__ __forceinline__ PagedItem paged_locate(const PagedAttnArgs &a, uint32_t which, int lane, uint32_t sub = 0)
+{
+    PagedItem it{};
+    it.run = paged_run(a.deal, a.deal.target ? paged_all_steps(a, lane) : 0.f);
+    uint32_t before = 0;
+    for (uint32_t b0 = 0; b0 < a.deal.seqs; b0 += 64) {
+        PagedSeq s{};
+        uint32_t tiles = 0, parts = 1;
+        if (b0 + lane < a.deal.seqs) {
+            s = paged_seq_of(a, b0 + lane);
+            tiles = paged_tiles(a.deal, s);
+            parts = paged_parts(paged_steps(a.deal, s), it.run);
+        }
+        const uint32_t upto = before + wave_running_sum_u32(tiles * parts);
+        const uint64_t here = __ballot(BY_ROW ? which >= s.row0 && which - s.row0 < s.rows : upto > which);
+        if (here) {
+            const int l = __builtin_ctzll(here);
+            const uint32_t n = __builtin_amdgcn_readlane(tiles, l);
+            it.seq = b0 + l;
+            it.parts = __builtin_amdgcn_readlane(parts, l);
+            it.s.row0 = __builtin_amdgcn_readlane(s.row0, l);
+            it.s.rows = __builtin_amdgcn_readlane(s.rows, l);
+            it.s.pos0 = (int32_t)__builtin_amdgcn_readlane((uint32_t)s.pos0, l);
+            it.s.keys = __builtin_amdgcn_readlane(s.keys, l);
+            it.any = true;
+            const uint32_t start = __builtin_amdgcn_readlane(upto, l) - n * it.parts;
+            // tiles that see most go first
+            const uint32_t back = BY_ROW ? n - 1 - ((which - it.s.row0) * a.deal.group + sub) / a.deal.tile : (which - start) / it.parts;
+            it.tile = n - 1 - back;
+            it.first = start + back * it.parts;
+            it.part = BY_ROW ? 0 : which - it.first;
+            return it;
+        }
+        before = __builtin_amdgcn_readlane(upto, 63);
+    }
+    return it;
+}
+
+// ---- elements ----------------------------------------------------------------------------------------------------------------------
+__device__ __forceinline__ float pg_bf16(uint32_t h) { return __uint_as_float(h << 16); }
+__device__ __forceinline__ float pg_exp2(float x) { return __builtin_amdgcn_exp2f(x); }      // 1 ulp; 0 below 2^-126
+
+// eight elements of `type` from `at` on
+__device__ __forceinline__ void pg_load8(const void *p, uint32_t type, uint64_t at, float (&x)[8])
+{
+    if (type == LV_F32) {
+        const float4 *f = reinterpret_cast<const float4 *>(static_cast<const float *>(p) + at);
+        const float4 u = f[0], v = f[1];
+        x[0] = u.x; x[1] = u.y; x[2] = u.z; x[3] = u.w; x[4] = v.x; x[5] = v.y; x[6] = v.z; x[7] = v.w;
+        return;
+    }
+    const uint4 u = *reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(p) + at);
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        x[2 * i] = type == LV_F16 ? half_bits_to_float((uint16_t)w[i]) : pg_bf16(w[i] & 0xffffu);
+        x[2 * i + 1] = type == LV_F16 ? half_bits_to_float((uint16_t)(w[i] >> 16)) : __uint_as_float(w[i] & 0xffff0000u);
+    }
+}
+__device__ __forceinline__ uint32_t pg_bits(float x, uint32_t type)
+{
+    return type == LV_F16 ? (uint32_t)float_to_half_bits(x) : (uint32_t)__builtin_bit_cast(uint16_t, (__bf16)x);
+}
+__device__ __forceinline__ void pg_store8(void *p, uint32_t type, uint64_t at, const float (&x)[8])
+{
+    if (type == LV_F32) {
+        float4 *f = reinterpret_cast<float4 *>(static_cast<float *>(p) + at);
+        f[0] = make_float4(x[0], x[1], x[2], x[3]);
+        f[1] = make_float4(x[4], x[5], x[6], x[7]);
+        return;
+    }
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) w[i] = pg_bits(x[2 * i], type) | (pg_bits(x[2 * i + 1], type) << 16);
+    *reinterpret_cast<uint4 *>(static_cast<uint16_t *>(p) + at) = make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// codes to fp16: the byte under 0x64 is 1024 + byte
+__device__ __forceinline__ uint32_t pg_pk_add(uint32_t a, float b)
+{
+    const pg_h2 r = __builtin_bit_cast(pg_h2, a) + pg_h2{(_Float16)b, (_Float16)b};
+    return __builtin_bit_cast(uint32_t, r);
+}
+__device__ __forceinline__ uint32_t pg_pk_mul(uint32_t a, pg_h2 d) { return __builtin_bit_cast(uint32_t, __builtin_bit_cast(pg_h2, a) * d); }
+// four bytes 0 .. 255 minus `bias`, as four fp16
+__device__ __forceinline__ void pg_bytes_to_half(uint32_t w, float bias, uint32_t &lo, uint32_t &hi)
+{
+    lo = pg_pk_add(__builtin_amdgcn_perm(0x64646464u, w, 0x04010400u), -1024.f - bias);
+    hi = pg_pk_add(__builtin_amdgcn_perm(0x64646464u, w, 0x04030402u), -1024.f - bias);
+}
+
+template <bool BF> struct PgFrag { typedef pg_h8 type; };
+template <> struct PgFrag<true> { typedef pg_b8 type; };
+template <bool BF> __device__ __forceinline__ pg_f4 pg_mfma(typename PgFrag<BF>::type a, typename PgFrag<BF>::type b, pg_f4 c)
+{
+    if constexpr (BF) return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+    else return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+}
+// x as a sum of N numbers of 16 bits: fp16 11 bits each, bf16 8
+template <bool BF, int N, class Frag> __device__ __forceinline__ void pg_cut(float x, int e, Frag (&f)[N])
+{
+#pragma unroll
+    for (int n = 0; n < N; n++) {
+        if constexpr (BF) {
+            const __bf16 h = (__bf16)x;
+            f[n][e] = h;
+            x -= (float)h;
+        } else {
+            const _Float16 h = (_Float16)x;
+            f[n][e] = h;
+            x -= (float)h;
+        }
+    }
+}
+
+// the columns of a 4 x 16 tile of 16-bit elements; each of 16 lanes names the 8 bytes at row lane / 4, columns 4 (lane % 4) ..
+__device__ __forceinline__ pg_s4 pg_read_columns(const uint8_t *p)
+{
+    typedef __attribute__((address_space(3))) pg_s4 lds_s4;
+    return __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4 *)p);
+}
+
+// ---- rows: single tokens, drafts, 32-bit queries -----------------------------------------------------------------------------------
+// A workgroup's tile is 16 QT rows; its four waves take turns of 32 keys and never wait for one another before the end, where their results are put
+// together.  Keys go from memory to registers as the first operand, values through the wave's own 32 rows of LDS; the next turn's are asked
+// for before this turn's are used.  Bound by the bytes of the cache.
+//
+// NQ: pieces of a query, 1, or with 32-bit queries 2 (fp16 rows: 22 bits) or 3 (bf16 rows: 24 bits); the weights have as many, 2 of bf16 at least.  Rows of
+// codes: keys enter as exact integers, a block's sum is scaled in fp32.  Values are scaled in fp16 (a rounding of 2^-11 of each, beside the 16-bit result's own); with
+// 32-bit queries they enter as two fp16 pieces, which hold them exactly: 19 bits at most, the last of them 2^-24 or more, as the scale's is.
+template <int D, int CT, int NQ, int QT>
+__global__ __launch_bounds__(256) void paged_rows_kernel(PagedAttnArgs a)
+{
+    constexpr bool BF = CT == kPgBf16, BLOCKS = CT == kPgQ8 || CT == kPgQ4, EXACT = NQ > 1;
+    constexpr int KS = D / 32, DT = D / 16, CH = D / 8, SW = CH < 16 ? CH - 1 : 15, NP = BF && NQ == 1 ? 2 : NQ, TILE = 16 * QT;
+    constexpr float kLift = BF ? 0.f : 12.f;
+    constexpr int MERGE = D + 4;                      // floats of a row of results in LDS
+    typedef typename PgFrag<BF>::type Frag;
+    constexpr int PLANES = BLOCKS && EXACT ? 2 : 1, VALUES = 32 * D * 2 * PLANES;      // bytes of a wave's 32 rows of values
+    __shared__ __attribute__((aligned(128))) uint8_t lds[4 * VALUES > 4 * 16 * MERGE * 4 ? 4 * VALUES : 4 * 16 * MERGE * 4];      // at the end 16 rows of results of each wave
+    __shared__ float ml[4][TILE][2];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l16 = lane & 15, g4 = lane >> 4;
+    const uint32_t head = blockIdx.x % a.c.kv_heads, item = blockIdx.x / a.c.kv_heads;
+    const PagedItem it = paged_locate<false>(a, item, lane);
+    if (!it.any) return;
+    const uint32_t group = a.deal.group, rows = it.s.rows * group, r0 = it.tile * TILE;
+    const uint32_t psize = 1u << a.c.shift;
+
+    // this lane's rows
+    Frag q[QT][KS][NQ];
+    float factor[QT];
+    int32_t lo[QT], hi[QT];
+#pragma unroll
+    for (int i = 0; i < QT; i++) {
+        const uint32_t r = r0 + i * 16 + l16;
+        const bool mine = r < rows;
+        const uint32_t t = mine ? r / group : 0, h = head * group + (mine ? r - t * group : 0);
+        const int32_t p = it.s.pos0 + (int32_t)t;
+        hi[i] = mine ? p : -1;
+        lo[i] = p >= 0 ? (int32_t)paged_first_key((uint32_t)p, a.deal.window, a.deal.chunk) : 0;
+        float x[KS][8], top = 0.f;
+        const uint64_t at = (uint64_t)(it.s.row0 + t) * a.ldq + (uint64_t)h * D;
+#pragma unroll
+        for (int k = 0; k < KS; k++) {
+            if constexpr (CT == kPgQ4) {      // byte 4 g + j of a block holds elements 4 g + j and 16 + 4 g + j
+                float u[8], v[8];
+                pg_load8(a.q, a.type, at + k * 32 + (g4 / 2) * 8, u);
+                pg_load8(a.q, a.type, at + k * 32 + 16 + (g4 / 2) * 8, v);
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    x[k][e] = g4 & 1 ? u[4 + e] : u[e];
+                    x[k][4 + e] = g4 & 1 ? v[4 + e] : v[e];
+                }
+            } else {
+                pg_load8(a.q, a.type, at + k * 32 + g4 * 8, x[k]);
+            }
+#pragma unroll
+            for (int e = 0; e < 8; e++) top = fmaxf(top, fabsf(x[k][e]));
+        }
+        top = fmaxf(top, __shfl_xor(top, 16, 64));
+        top = fmaxf(top, __shfl_xor(top, 32, 64));
+        // a power of two brings the row's largest element to 2^10 .. 2^11: no overflow, and small pieces are no subnormals
+        int e2 = (int)(__float_as_uint(top) >> 23) - 127 - 10;
+        if (e2 > 117 || e2 < -110) e2 = 0;      // inf, NaN; 0 and numbers next to it
+        const float down = __uint_as_float((uint32_t)(127 - e2) << 23);
+        factor[i] = a.scale * __uint_as_float((uint32_t)(127 + e2) << 23);
+#pragma unroll
+        for (int k = 0; k < KS; k++)
+#pragma unroll
+            for (int e = 0; e < 8; e++) pg_cut<BF, NQ>(mine ? x[k][e] * down : 0.f, e, q[i][k]);
+    }
+    // keys that any row sees, and those that all rows see
+    const uint32_t last_row = min(r0 + TILE, rows) - 1;
+    const int32_t p_first = it.s.pos0 + (int32_t)(r0 / group), p_last = it.s.pos0 + (int32_t)(last_row / group);
+    const uint32_t k_lo = p_first >= 0 ? paged_first_key((uint32_t)p_first, a.deal.window, a.deal.chunk) : 0;
+    const uint32_t k_hi = p_last >= 0 ? min((uint32_t)p_last + 1, it.s.keys) : 0;
+    const uint32_t all_lo = p_last >= 0 ? paged_first_key((uint32_t)p_last, a.deal.window, a.deal.chunk) : 0, all_hi = p_first >= 0 ? (uint32_t)p_first + 1 : 0;
+    const uint32_t base = k_lo & ~31u, n_steps = k_hi > base ? (k_hi - base + kPagedStep - 1) / kPagedStep : 0;
+    const uint32_t s0 = min((uint64_t)it.part * it.run, (uint64_t)n_steps), s1 = min((uint64_t)s0 + it.run, (uint64_t)n_steps);
+
+    const uint32_t *table = a.table + (uint64_t)it.seq * a.table_ld;
+    const uint32_t turns = n_steps ? (k_hi - base + 31) / 32 : 0, t_end = min(s1 * 4, turns);
+    uint8_t *mine = lds + wave * VALUES;
+
+    struct Turn {
+        uint4 k4[CT <= kPgBf16 ? 2 : 1][CT <= kPgBf16 ? KS : 1];
+        uint2 k2[CT == kPgQ8 ? 2 : 1][CT == kPgQ8 ? KS : 1];
+        uint32_t k1[CT == kPgQ4 ? 2 : 1][CT == kPgQ4 ? KS : 1];
+        uint2 ks[BLOCKS ? 2 : 1][BLOCKS ? KS : 1];                          // scales of keys 4 g .. 4 g + 3 of 16: [key][block]
+        uint4 v4[CT <= kPgBf16 ? D / 16 : CT == kPgQ8 ? D / 32 : 1];        // 16 bytes of a row
+        uint2 v2[CT == kPgQ4 ? D / 32 : 1];                                 // 8 bytes: half a block's
+        uint16_t vd[BLOCKS ? D / 32 : 1];
+        bool ok[2];                                                         // 16 keys each: is there a page?
+    };
+    // row of 32 and unit of the row that this lane brings with its i-th load of values
+    constexpr int UNITS = CT <= kPgBf16 ? CH : D / 16, LOADS = 32 * UNITS / 64;
+    auto row_of = [&](int i) { return (i * 64 + lane) / UNITS; };
+    auto unit_of = [&](int i) { return (i * 64 + lane) % UNITS; };
+    auto load = [&](Turn &x, uint32_t t) {
+        const uint32_t kb = base + t * 32;
+        const uint8_t *pk[2], *pv[2], *pks[2], *pvs[2];
+#pragma unroll
+        for (int kt = 0; kt < 2; kt++) {
+            const uint32_t at = kb + 16 * kt, page = paged_page(a.c, table, a.table_ld, at), in = at & (psize - 1);
+            x.ok[kt] = page != kNoPage;
+            const uint8_t *block = a.c.data + ((uint64_t)(x.ok[kt] ? page : 0) * a.c.kv_heads + head) * a.c.block;
+            pk[kt] = block + in * a.c.code_row;
+            pv[kt] = pk[kt] + a.c.half;
+            pks[kt] = block + (a.c.code_row << a.c.shift) + in * a.c.scale_row;
+            pvs[kt] = pks[kt] + a.c.half;
+        }
+#pragma unroll
+        for (int kt = 0; kt < 2; kt++)
+#pragma unroll
+            for (int k = 0; k < KS; k++) {
+                if constexpr (CT <= kPgBf16) x.k4[kt][k] = *reinterpret_cast<const uint4 *>(pk[kt] + (uint32_t)(l16 * (2 * D) + k * 64 + g4 * 16));
+                else if constexpr (CT == kPgQ8) x.k2[kt][k] = *reinterpret_cast<const uint2 *>(pk[kt] + (uint32_t)(l16 * D + k * 32 + g4 * 8));
+                else x.k1[kt][k] = *reinterpret_cast<const uint32_t *>(pk[kt] + (uint32_t)(l16 * (D / 2) + k * 16 + g4 * 4));
+                if constexpr (BLOCKS) x.ks[kt][k] = *reinterpret_cast<const uint2 *>(pks[kt] + (uint32_t)(g4 * (D / 4) + k * 8));
+            }
+#pragma unroll
+        for (int i = 0; i < LOADS; i++) {
+            const int row = row_of(i), u = unit_of(i);
+            const uint8_t *p = row < 16 ? pv[0] : pv[1];
+            if constexpr (CT <= kPgBf16) x.v4[i] = *reinterpret_cast<const uint4 *>(p + (uint32_t)((row & 15) * (2 * D) + u * 16));
+            else if constexpr (CT == kPgQ8) x.v4[i] = *reinterpret_cast<const uint4 *>(p + (uint32_t)((row & 15) * D + u * 16));
+            else x.v2[i] = *reinterpret_cast<const uint2 *>(p + (uint32_t)((row & 15) * (D / 2) + u * 8));
+            if constexpr (BLOCKS) x.vd[i] = *reinterpret_cast<const uint16_t *>((row < 16 ? pvs[0] : pvs[1]) + (uint32_t)((row & 15) * (D / 16) + u / 2 * 2));
+        }
+    };
+
+    pg_f4 o[DT][QT];
+    float m[QT], l[QT];
+#pragma unroll
+    for (int i = 0; i < QT; i++) {
+        m[i] = -1e30f;
+        l[i] = 0.f;
+#pragma unroll
+        for (int d = 0; d < DT; d++) o[d][i] = pg_f4{0.f, 0.f, 0.f, 0.f};
+    }
+    // eight elements into chunk `ch` of a row of values in LDS
+    auto put = [&](int row, int ch, uint4 w, int plane = 0) { *reinterpret_cast<uint4 *>(mine + plane * (32 * D * 2) + row * (2 * D) + ((ch ^ (row & SW)) * 16)) = w; };
+    // first operand of O^T for dimensions 16 d ..: dimension l16, keys 4 g .. + 3 and 16 + 4 g .. + 3
+    auto values = [&](int d, int plane = 0) {
+        const int row = 4 * g4 + l16 / 4, c = 16 * d + 4 * (l16 & 3);
+        const int off = (c % 8) * 2 + plane * (32 * D * 2);
+        const pg_s4 u = pg_read_columns(mine + row * (2 * D) + (((c / 8) ^ (row & SW)) * 16) + off);
+        const pg_s4 v = pg_read_columns(mine + (row + 16) * (2 * D) + (((c / 8) ^ ((row + 16) & SW)) * 16) + off);
+        return __builtin_bit_cast(Frag, pg_s8{u[0], u[1], u[2], u[3], v[0], v[1], v[2], v[3]});
+    };
+
+    auto use = [&](Turn &x, uint32_t t) {
+        const uint32_t kb = base + t * 32;
+        const bool inside = kb >= k_lo && kb + 32 <= k_hi && x.ok[0] && x.ok[1];        // every key of the turn is some row's
+        const bool edge = kb < all_lo || kb + 32 > all_hi || !inside;                   // some row does not see all of them
+        auto sees = [&](int i, int kt, int r) {
+            const int32_t p = (int32_t)(kb + kt * 16 + g4 * 4 + r);
+            return p >= lo[i] && p <= hi[i] && p < (int32_t)k_hi && x.ok[kt];
+        };
+        pg_f4 sc[2][QT];
+#pragma unroll
+        for (int kt = 0; kt < 2; kt++) {
+#pragma unroll
+            for (int i = 0; i < QT; i++) sc[kt][i] = pg_f4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int k = 0; k < KS; k++) {
+                Frag f;
+                if constexpr (CT <= kPgBf16) {
+                    f = __builtin_bit_cast(Frag, x.k4[kt][k]);
+                } else {
+                    uint4 w;
+                    if constexpr (CT == kPgQ8) {
+                        pg_bytes_to_half(x.k2[kt][k].x ^ 0x80808080u, 128.f, w.x, w.y);
+                        pg_bytes_to_half(x.k2[kt][k].y ^ 0x80808080u, 128.f, w.z, w.w);
+                    } else {
+                        pg_bytes_to_half(x.k1[kt][k] & 0x0f0f0f0fu, 8.f, w.x, w.y);
+                        pg_bytes_to_half((x.k1[kt][k] >> 4) & 0x0f0f0f0fu, 8.f, w.z, w.w);
+                    }
+                    f = __builtin_bit_cast(Frag, w);
+                }
+#pragma unroll
+                for (int i = 0; i < QT; i++) {
+                    pg_f4 acc = BLOCKS ? pg_f4{0.f, 0.f, 0.f, 0.f} : sc[kt][i];
+#pragma unroll
+                    for (int n = NQ - 1; n >= 0; n--) acc = pg_mfma<BF>(f, q[i][k][n], acc);
+                    if constexpr (BLOCKS) {
+#pragma unroll
+                        for (int r = 0; r < 4; r++) {
+                            const int at = r * KS + k;      // half at / of ks: [key][block]
+                            const uint32_t word = at % 4 < 2 ? x.ks[kt][at / 4].x : x.ks[kt][at / 4].y;
+                            sc[kt][i][r] = fmaf(half_bits_to_float((uint16_t)(word >> (at % 2 * 16))), acc[r], sc[kt][i][r]);
+                        }
+                    } else {
+                        sc[kt][i] = acc;
+                    }
+                }
+            }
+        }
+        Frag p[QT][NP];
+#pragma unroll
+        for (int i = 0; i < QT; i++) {
+            float s[8], top = m[i];
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                s[e] = sc[e / 4][i][e % 4] * factor[i];
+                if (edge && !sees(i, e / 4, e % 4)) s[e] = -INFINITY;
+                top = fmaxf(top, s[e]);
+            }
+            top = fmaxf(top, __shfl_xor(top, 16, 64));
+            top = fmaxf(top, __shfl_xor(top, 32, 64));
+            if (__any(top > m[i])) {
+                const float f = pg_exp2(m[i] - top);
+                m[i] = top;
+                l[i] *= f;
+#pragma unroll
+                for (int d = 0; d < DT; d++)
+#pragma unroll
+                    for (int r = 0; r < 4; r++) o[d][i][r] *= f;
+            }
+            float sum = 0.f;
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                const float w = pg_exp2(s[e] - m[i] + kLift);
+                sum += w;
+                pg_cut<BF, NP>(w, e, p[i]);
+            }
+            l[i] += sum;
+        }
+        // Values that no row sees are made 0: a page's rows behind the sequence's end may hold anything, and 0 times that has to be 0.  Numbers that are not
+        // finite are taken out and added apart to the rows that see them: a weight that is 0, or a negative piece of one, would spread them or turn their sign.
+        if (!inside) {
+#pragma unroll
+            for (int i = 0; i < LOADS; i++) {
+                const int row = row_of(i);
+                const bool keep = kb + row >= k_lo && kb + row < k_hi && (row < 16 ? x.ok[0] : x.ok[1]);
+                if constexpr (CT <= kPgBf16) {
+                    if (!keep) x.v4[i] = make_uint4(0, 0, 0, 0);
+                } else {
+                    if (!keep) x.vd[i] = 0;
+                }
+            }
+        }
+        if constexpr (CT <= kPgBf16) {
+            constexpr uint32_t EXP = BF ? 0x7f807f80u : 0x7c007c00u, ONE = BF ? 0x00800080u : 0x04000400u;
+            uint32_t odd = 0;
+#pragma unroll
+            for (int i = 0; i < LOADS; i++)
+                odd |= (((x.v4[i].x & EXP) + ONE) | ((x.v4[i].y & EXP) + ONE) | ((x.v4[i].z & EXP) + ONE) | ((x.v4[i].w & EXP) + ONE)) & 0x80008000u;
+            if (__any(odd != 0)) {
+                // 0: NaN, 1: inf, 2: -inf.  Counts of each among the keys a row sees, as a product of ones
+                for (int kind = 0; kind < 3; kind++) {
+                    auto count = [&](uint32_t w) {
+                        uint32_t out = 0;
+#pragma unroll
+                        for (int e = 0; e < 2; e++) {
+                            const uint32_t h = (w >> (16 * e)) & 0xffffu, ex = EXP & 0xffffu;
+                            const bool special = (h & ex) == ex, nan = special && (h & 0x7fffu) != ex;
+                            const bool yes = kind == 0 ? nan : special && !nan && (h >> 15) == (uint32_t)(kind - 1);
+                            out |= yes ? (BF ? 0x3f80u : 0x3c00u) << (16 * e) : 0u;
+                        }
+                        return out;
+                    };
+#pragma unroll
+                    for (int i = 0; i < LOADS; i++) put(row_of(i), unit_of(i), make_uint4(count(x.v4[i].x), count(x.v4[i].y), count(x.v4[i].z), count(x.v4[i].w)));
+                    const float add = kind == 0 ? __builtin_nanf("") : kind == 1 ? INFINITY : -INFINITY;
+#pragma unroll
+                    for (int i = 0; i < QT; i++) {
+                        Frag one;
+#pragma unroll
+                        for (int e = 0; e < 8; e++) {
+                            const float s = sees(i, e / 4, e % 4) ? 1.f : 0.f;
+                            if constexpr (BF) one[e] = (__bf16)s;
+                            else one[e] = (_Float16)s;
+                        }
+#pragma unroll
+                        for (int d = 0; d < DT; d++) {
+                            const pg_f4 n = pg_mfma<BF>(values(d), one, pg_f4{0.f, 0.f, 0.f, 0.f});
+#pragma unroll
+                            for (int r = 0; r < 4; r++) o[d][i][r] += n[r] > 0.f ? add : 0.f;
+                        }
+                    }
+                }
+                auto finite = [&](uint32_t w) {
+                    const uint32_t ex = EXP & 0xffffu;
+                    return (((w & ex) == ex) ? 0u : w & 0xffffu) | ((((w >> 16) & ex) == ex) ? 0u : w & 0xffff0000u);
+                };
+#pragma unroll
+                for (int i = 0; i < LOADS; i++) x.v4[i] = make_uint4(finite(x.v4[i].x), finite(x.v4[i].y), finite(x.v4[i].z), finite(x.v4[i].w));
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < LOADS; i++) {
+            const int row = row_of(i), u = unit_of(i);
+            if constexpr (CT <= kPgBf16) {
+                put(row, u, x.v4[i]);
+            } else {
+                uint4 w0, w1;
+                if constexpr (CT == kPgQ8) {
+                    pg_bytes_to_half(x.v4[i].x ^ 0x80808080u, 128.f, w0.x, w0.y);
+                    pg_bytes_to_half(x.v4[i].y ^ 0x80808080u, 128.f, w0.z, w0.w);
+                    pg_bytes_to_half(x.v4[i].z ^ 0x80808080u, 128.f, w1.x, w1.y);
+                    pg_bytes_to_half(x.v4[i].w ^ 0x80808080u, 128.f, w1.z, w1.w);
+                } else {
+                    pg_bytes_to_half(x.v2[i].x & 0x0f0f0f0fu, 8.f, w0.x, w0.y);
+                    pg_bytes_to_half(x.v2[i].y & 0x0f0f0f0fu, 8.f, w0.z, w0.w);
+                    pg_bytes_to_half((x.v2[i].x >> 4) & 0x0f0f0f0fu, 8.f, w1.x, w1.y);
+                    pg_bytes_to_half((x.v2[i].y >> 4) & 0x0f0f0f0fu, 8.f, w1.z, w1.w);
+                }
+                const _Float16 d = __builtin_bit_cast(_Float16, x.vd[i]);
+                const int c0 = CT == kPgQ8 ? 2 * u : u / 2 * 4 + u % 2, c1 = CT == kPgQ8 ? c0 + 1 : c0 + 2;
+                if constexpr (EXACT) {
+                    auto cut = [&](uint4 w, int ch) {
+                        const pg_h8 code = __builtin_bit_cast(pg_h8, w);
+                        pg_h8 piece[2];
+#pragma unroll
+                        for (int e = 0; e < 8; e++) pg_cut<false, 2>((float)code[e] * (float)d, e, piece);
+                        put(row, ch, __builtin_bit_cast(uint4, piece[0]));
+                        put(row, ch, __builtin_bit_cast(uint4, piece[1]), 1);
+                    };
+                    cut(w0, c0);
+                    cut(w1, c1);
+                } else {
+                    const pg_h2 dd = {d, d};
+                    put(row, c0, make_uint4(pg_pk_mul(w0.x, dd), pg_pk_mul(w0.y, dd), pg_pk_mul(w0.z, dd), pg_pk_mul(w0.w, dd)));
+                    put(row, c1, make_uint4(pg_pk_mul(w1.x, dd), pg_pk_mul(w1.y, dd), pg_pk_mul(w1.z, dd), pg_pk_mul(w1.w, dd)));
+                }
+            }
+        }
+#pragma unroll
+        for (int d = 0; d < DT; d++) {
+            if constexpr (PLANES == 2) {      // the smaller pieces first; the product of both smaller ones is 2^-22 of the whole
+                const Frag v = values(d, 1);
+#pragma unroll
+                for (int i = 0; i < QT; i++) o[d][i] = pg_mfma<BF>(v, p[i][0], o[d][i]);
+            }
+            const Frag v = values(d);
+#pragma unroll
+            for (int i = 0; i < QT; i++)
+#pragma unroll
+                for (int n = NP - 1; n >= 0; n--) o[d][i] = pg_mfma<BF>(v, p[i][n], o[d][i]);
+        }
+    };
+
+    uint32_t t = s0 * 4 + wave;
+    Turn x;
+    if (t < t_end) load(x, t);
+    while (t < t_end) {
+        Turn next = x;
+        if (t + 4 < t_end) load(next, t + 4);
+        use(x, t);
+        x = next;
+        t += 4;
+    }
+
+    // the four waves' results put together, 16 rows at a time
+#pragma unroll
+    for (int i = 0; i < QT; i++) {
+        float sum = l[i];
+        sum += __shfl_xor(sum, 16, 64);
+        sum += __shfl_xor(sum, 32, 64);
+        if (g4 == 0) {
+            ml[wave][i * 16 + l16][0] = m[i];
+            ml[wave][i * 16 + l16][1] = sum;
+        }
+    }
+    float *res = reinterpret_cast<float *>(lds);
+#pragma unroll
+    for (int i = 0; i < QT; i++) {
+        __syncthreads();      // ml, and the values of all waves are read; then the 16 rows before these
+        float top = ml[0][i * 16 + l16][0];
+#pragma unroll
+        for (int w = 1; w < 4; w++) top = fmaxf(top, ml[w][i * 16 + l16][0]);
+        const float f = pg_exp2(m[i] - top);
+#pragma unroll
+        for (int d = 0; d < DT; d++)
+            *reinterpret_cast<float4 *>(res + (wave * 16 + l16) * MERGE + d * 16 + g4 * 4) = make_float4(o[d][i][0] * f, o[d][i][1] * f, o[d][i][2] * f, o[d][i][3] * f);
+        __syncthreads();
+        for (int u = threadIdx.x; u < 16 * CH; u += 256) {
+            const int row = u / CH, c = u % CH * 8;
+            const uint32_t r = r0 + i * 16 + row;
+            if (r >= rows) continue;
+            float y[8], ms[4];
+#pragma unroll
+            for (int e = 0; e < 8; e++) y[e] = 0.f;
+            float big = -1e30f, all = 0.f;
+#pragma unroll
+            for (int w = 0; w < 4; w++) {
+                ms[w] = ml[w][i * 16 + row][0];
+                big = fmaxf(big, ms[w]);
+                const float4 *s = reinterpret_cast<const float4 *>(res + (w * 16 + row) * MERGE + c);
+                y[0] += s[0].x; y[1] += s[0].y; y[2] += s[0].z; y[3] += s[0].w;
+                y[4] += s[1].x; y[5] += s[1].y; y[6] += s[1].z; y[7] += s[1].w;
+            }
+#pragma unroll
+            for (int w = 0; w < 4; w++) all = fmaf(ml[w][i * 16 + row][1], pg_exp2(ms[w] - big), all);
+            if (it.parts > 1) {
+                const uint64_t at = ((uint64_t)item * a.c.kv_heads + head) * TILE + i * 16 + row;
+                pg_store8(a.part, LV_F32, at * D + c, y);
+                if (c == 0) {
+                    a.part_ml[2 * at] = big;
+                    a.part_ml[2 * at + 1] = all;
+                }
+                continue;
+            }
+            const uint32_t t2 = r / group, h = head * group + (r - t2 * group);
+            float f2 = 1.f;
+            if (a.sinks) {
+                const float sink = a.sinks[h] * 1.44269504088896341f, over = fmaxf(big, sink);
+                f2 = pg_exp2(big - over);
+                all = fmaf(all, f2, pg_exp2(sink - over + kLift));
+            }
+            f2 = all == 0.f ? 0.f : f2 / all;
+#pragma unroll
+            for (int e = 0; e < 8; e++) y[e] = all == 0.f ? 0.f : y[e] * f2;
+            pg_store8(a.out, a.type, (uint64_t)(it.s.row0 + t2) * a.ldo + (uint64_t)h * D + c, y);
+        }
+    }
+}
+
+// ---- the parts of cut items put together: a workgroup a row ------------------------------------------------------------------------
+template <int D>
+__global__ __launch_bounds__(256) void paged_join_kernel(PagedAttnArgs a, float lift)
+{
+    __shared__ float sums[4][D], tops[4][2];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t heads = a.c.kv_heads * a.deal.group, row = blockIdx.x / heads, h = blockIdx.x % heads;
+    const PagedItem it = paged_locate<true>(a, row, lane, h % a.deal.group);
+    if (!it.any || it.parts == 1) return;
+    const uint32_t group = a.deal.group, kvh = h / group, r = (row - it.s.row0) * group + h % group, in = r - it.tile * a.deal.tile;
+    // wave w takes parts w, w + 4, ..
+    constexpr int V = D >= 64 ? D / 64 : 1;
+    const bool mine = lane * V < D;
+    float top = -1e30f, all = 0.f, y[V];
+#pragma unroll
+    for (int e = 0; e < V; e++) y[e] = 0.f;
+    for (uint32_t p0 = wave; p0 < it.parts; p0 += 16) {
+        float ms[4], ls[4], v[4][V];
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const uint32_t p = p0 + 4 * j;
+            const uint64_t at = ((uint64_t)(it.first + min(p, it.parts - 1)) * a.c.kv_heads + kvh) * a.deal.tile + in;
+            ms[j] = a.part_ml[2 * at];
+            ls[j] = a.part_ml[2 * at + 1];
+            if (p >= it.parts) {
+                ms[j] = -1e30f;
+                ls[j] = 0.f;
+            }
+#pragma unroll
+            for (int e = 0; e < V; e++) v[j][e] = mine && p < it.parts ? a.part[at * D + lane * V + e] : 0.f;
+        }
+        const float big = fmaxf(fmaxf(fmaxf(ms[0], ms[1]), fmaxf(ms[2], ms[3])), top), f = pg_exp2(top - big);
+        top = big;
+        all *= f;
+#pragma unroll
+        for (int e = 0; e < V; e++) y[e] *= f;
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const float g = pg_exp2(ms[j] - big);
+            all = fmaf(ls[j], g, all);
+#pragma unroll
+            for (int e = 0; e < V; e++) y[e] = fmaf(v[j][e], g, y[e]);
+        }
+    }
+#pragma unroll
+    for (int e = 0; e < V; e++)
+        if (mine) sums[wave][lane * V + e] = y[e];
+    if (lane == 0) {
+        tops[wave][0] = top;
+        tops[wave][1] = all;
+    }
+    __syncthreads();
+    if (threadIdx.x >= D / 8) return;
+    float big = fmaxf(fmaxf(tops[0][0], tops[1][0]), fmaxf(tops[2][0], tops[3][0]));
+    const float sink = a.sinks ? a.sinks[h] * 1.44269504088896341f : -1e30f;
+    big = fmaxf(big, sink);
+    float total = a.sinks ? pg_exp2(sink - big + lift) : 0.f, z[8];
+#pragma unroll
+    for (int e = 0; e < 8; e++) z[e] = 0.f;
+#pragma unroll
+    for (int w = 0; w < 4; w++) {
+        const float g = pg_exp2(tops[w][0] - big);
+        total = fmaf(tops[w][1], g, total);
+#pragma unroll
+        for (int e = 0; e < 8; e++) z[e] = fmaf(sums[w][threadIdx.x * 8 + e], g, z[e]);
+    }
+    const float f = 1.f / total;
+#pragma unroll
+    for (int e = 0; e < 8; e++) z[e] = total == 0.f ? 0.f : z[e] * f;
+    pg_store8(a.out, a.type, (uint64_t)row * a.ldo + (uint64_t)h * D + threadIdx.x * 8, z);
+}
+
+}  // namespace lv

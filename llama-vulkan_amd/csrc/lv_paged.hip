@@ -1,0 +1,119 @@
+// lv_paged.hip — lv_kernel_paged_attention: which kernel a call takes, and its launches.
+#include <cmath>
+
+#include "lv_paged.h"
+#include "lv_serve_host.h"
+
+using namespace lv;
+
+namespace {
+
+struct AttnPlan {
+    PagedAttnArgs args{};
+    uint32_t tiles;                  // of 16 rows a workgroup
+    uint32_t pieces;                 // of a query
+    uint64_t items, part_floats, bytes;
+};
+
+// Workgroups that share the work of a call.  
+constexpr uint32_t kTargetPerUnit = 4;
+
+AttnPlan attn_plan(uint32_t units, uint32_t type, const lv_paged_cache &c, const lv_paged_batch &b, const lv_paged_attn_spec &s)
+{
+    AttnPlan p;
+    PagedDeal &d = p.args.deal;
+    const uint32_t group = s.heads / c.kv_heads;
+    p.tiles = c.dim <= 128 && (uint64_t)b.tokens * group > 16ull * b.seqs ? 2 : 1;
+    p.pieces = type == LV_F32 ? (c.type == LV_BF16 ? 3 : 2) : type == LV_F16 && c.type == LV_BF16 ? 3 : 1;
+    d.seqs = b.seqs;
+    d.tokens = b.tokens;
+    d.group = group;
+    d.tile = 16 * p.tiles;
+    d.kv_heads = c.kv_heads;
+    d.window = s.window;
+    d.chunk = s.chunk;
+    d.positions = b.table_ld * c.page;
+    d.target = kTargetPerUnit * units;
+    if ((uint64_t)b.tokens * group / d.tile * c.kv_heads >= d.target) d.target = 0;
+    p.items = paged_items(d);
+    p.part_floats = d.target ? p.items * c.kv_heads * d.tile * c.dim : 0;
+    p.bytes = d.target ? (p.part_floats + p.items * c.kv_heads * d.tile * 2) * 4 : 0;
+    return p;
+}
+
+template <int D, int CT, int NQ>
+void launch_rows(const AttnPlan &p, uint32_t grid, hipStream_t st)
+{
+    if constexpr (D <= 128) {
+        if (p.tiles == 2) {
+            paged_rows_kernel<D, CT, NQ, 2><<<dim3(grid), dim3(256), 0, st>>>(p.args);
+            return;
+        }
+    }
+    paged_rows_kernel<D, CT, NQ, 1><<<dim3(grid), dim3(256), 0, st>>>(p.args);
+}
+
+template <int D>
+void launch_attention(const AttnPlan &p, uint32_t grid, hipStream_t st)
+{
+    const PagedAttnArgs &a = p.args;
+    switch (a.c.type) {
+    case LV_F16: p.pieces == 1 ? launch_rows<D, kPgF16, 1>(p, grid, st) : launch_rows<D, kPgF16, 2>(p, grid, st); break;
+    case LV_BF16: p.pieces == 1 ? launch_rows<D, kPgBf16, 1>(p, grid, st) : launch_rows<D, kPgBf16, 3>(p, grid, st); break;
+    case LV_Q8_0: p.pieces == 1 ? launch_rows<D, kPgQ8, 1>(p, grid, st) : launch_rows<D, kPgQ8, 2>(p, grid, st); break;
+    default: p.pieces == 1 ? launch_rows<D, kPgQ4, 1>(p, grid, st) : launch_rows<D, kPgQ4, 2>(p, grid, st); break;
+    }
+    if (a.deal.target) paged_join_kernel<D><<<dim3(a.deal.tokens * a.deal.group * a.deal.kv_heads), dim3(256), 0, st>>>(a, a.c.type == LV_BF16 ? 0.f : 12.f);
+}
+
+}  // namespace
+
+extern "C" int lv_paged_attention_workspace(lv_ctx *c, uint32_t type, const lv_paged_cache *cache, const lv_paged_batch *batch, const lv_paged_attn_spec *spec,
+                                            uint64_t *bytes)
+{
+    if (!bytes) return fail(LV_ERR_ARG, "lv_paged_attention_workspace: bytes is null");
+    *bytes = 0;
+    if (const char *e = paged_attn_refusal(cache, batch, spec, type)) return fail(LV_ERR_ARG, "lv_paged_attention_workspace: %s", e);
+    if (!c) return fail(LV_ERR_ARG, "lv_paged_attention_workspace: ctx is null");
+    if (batch->seqs && batch->tokens) *bytes = attn_plan(ctx_units(c), type, *cache, *batch, *spec).bytes;
+    return LV_OK;
+}
+
+extern "C" int lv_kernel_paged_attention(lv_ctx *c, void *out, uint32_t ldo, const void *q, uint32_t ldq, uint32_t type, const lv_paged_cache *cache,
+                                         const lv_paged_batch *batch, const lv_paged_attn_spec *spec, void *work, uint64_t work_bytes)
+{
+    if (const char *e = paged_attn_rows_refusal(cache, batch, spec, type, out, ldo, q, ldq)) return fail(LV_ERR_ARG, "lv_kernel_paged_attention: %s", e);
+    if (!c) return fail(LV_ERR_ARG, "lv_kernel_paged_attention: ctx is null");
+    if (batch->seqs == 0 || batch->tokens == 0) return LV_OK;
+    AttnPlan p = attn_plan(ctx_units(c), type, *cache, *batch, *spec);
+    if (p.bytes && (!work || work_bytes < p.bytes || (uintptr_t)work % 16))
+        return fail(LV_ERR_ARG, "lv_kernel_paged_attention: a workspace of %llu bytes, aligned to 16, is needed", (unsigned long long)p.bytes);
+    const uint64_t grid = p.items * cache->kv_heads, rows = (uint64_t)batch->tokens * spec->heads;
+    if (grid > 0x7fffffffu || rows > 0x7fffffffu) return fail(LV_ERR_RANGE, "lv_kernel_paged_attention: %u tokens of %u heads", batch->tokens, spec->heads);
+    PagedAttnArgs &a = p.args;
+    a.c = paged_view(*cache);
+    a.starts = batch->starts;
+    a.lens = batch->lens;
+    a.table = batch->table;
+    a.table_ld = batch->table_ld;
+    a.q = q;
+    a.out = out;
+    a.ldq = ldq;
+    a.ldo = ldo;
+    a.type = type;
+    a.scale = spec->scale * 1.44269504088896341f;
+    a.sinks = spec->sinks;
+    a.part = static_cast<float *>(work);
+    a.part_ml = a.part + p.part_floats;
+    DeviceScope scope(ctx_device(c));
+    HIP_TRY(scope.error);
+    const hipStream_t st = ctx_stream(c);
+    switch (cache->dim) {
+    case 32: launch_attention<32>(p, (uint32_t)grid, st); break;
+    case 64: launch_attention<64>(p, (uint32_t)grid, st); break;
+    case 128: launch_attention<128>(p, (uint32_t)grid, st); break;
+    default: launch_attention<256>(p, (uint32_t)grid, st); break;
+    }
+    HIP_TRY(hipGetLastError());
+    return LV_OK;
+}

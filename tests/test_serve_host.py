@@ -1,0 +1,314 @@
+"""A serving step's operators without a GPU: what their entry points refuse, the cache's layout, which row lies where, and how attention is dealt to
+workgroups.  Refusals are asked of the library without a context: every argument is looked at before the context is."""
+import os
+import subprocess
+
+import numpy as np
+import pytest
+
+import serve_reference as ref
+
+CSRC = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "llama-vulkan_amd", "csrc")
+P = 4096      # an aligned pointer that nothing follows
+
+
+def cache(lva, **kw):
+    c = dict(data=P, type=lva.LV_F16, kv_heads=8, dim=128, page=16, pages=10)
+    c.update(kw)
+    return lva.PagedCache(*c.values())
+
+
+def batch(lva, **kw):
+    b = dict(seqs=2, tokens=5, starts=P, lens=P, table=P, table_ld=4)
+    b.update(kw)
+    return lva.PagedBatch(*b.values())
+
+
+def spec(lva, **kw):
+    s = dict(heads=32, scale=0.1, window=0, chunk=0, sinks=None)
+    s.update(kw)
+    return lva.PagedAttnSpec(*s.values())
+
+
+CACHES = [(dict(type=0), "type"), (dict(type=3), "type"), (dict(dim=96), "head size"), (dict(dim=0), "head size"), (dict(dim=512), "head size"), (dict(page=8), "page"),
+          (dict(page=48), "page"), (dict(page=2048), "page"), (dict(page=0), "page"), (dict(kv_heads=0), "kv_heads"), (dict(kv_heads=5000), "kv_heads"), (dict(pages=0), "pages")]
+POOLS = [(dict(data=None), "data"), (dict(data=P + 8), "aligned")]
+BATCHES = [(dict(seqs=70000), "sequences"), (dict(tokens=(1 << 24) + 1), "tokens"), (dict(table_ld=1 << 27), "2^30"), (dict(starts=None), "null"), (dict(lens=None), "null"),
+           (dict(table=None), "null"), (dict(starts=P + 2), "aligned"), (dict(lens=P + 1), "aligned"), (dict(table=P + 3), "aligned")]
+
+
+def refused(lva, rc, word):
+    text = lva.hip().lv_last_error().decode()
+    assert rc == -1 and word in text, (rc, text)
+
+
+@pytest.mark.parametrize("name", ["lv_kernel_paged_write", "lv_kernel_paged_read"])
+def test_rows_refusals(lva, name):
+    call = getattr(lva.hip(), name)
+    width = 8 * 128
+    for kw, word in CACHES + POOLS:
+        refused(lva, call(None, cache(lva, **kw), batch(lva), P, width, P, width, lva.LV_F32), word)
+    for kw, word in BATCHES:
+        refused(lva, call(None, cache(lva), batch(lva, **kw), P, width, P, width, lva.LV_F32), word)
+    ok = cache(lva), batch(lva)
+    refused(lva, call(None, None, ok[1], P, width, P, width, 0), "cache is null")
+    refused(lva, call(None, ok[0], None, P, width, P, width, 0), "batch is null")
+    refused(lva, call(None, *ok, P, width, P, width, lva.LV_Q8_0), "type")
+    refused(lva, call(None, *ok, None, width, P, width, 0), "null")
+    refused(lva, call(None, *ok, P, width, None, width, 0), "null")
+    refused(lva, call(None, *ok, P, width - 4, P, width, 0), "stride")
+    refused(lva, call(None, *ok, P, width, P, width - 4, 0), "stride")
+    refused(lva, call(None, *ok, P + 4, width, P, width, 0), "16 bytes")
+    refused(lva, call(None, *ok, P, width, P + 8, width, 0), "16 bytes")
+    refused(lva, call(None, *ok, P, width + 2, P, width, 0), "16 bytes")
+    refused(lva, call(None, *ok, P, width, P, width + 4, lva.LV_BF16), "16 bytes")
+    refused(lva, call(None, *ok, P, width, P, width, 0), "ctx")      # nothing else to refuse
+
+
+def test_attention_refusals(lva):
+    call, size = lva.hip().lv_kernel_paged_attention, lva.hip().lv_paged_attention_workspace
+    n = lva.C.c_uint64(7)
+
+    def both(c, b, s, kind, word):
+        refused(lva, call(None, P, 4096, P, 4096, kind, c, b, s, None, 0), word)
+        refused(lva, size(None, kind, c, b, s, n), word)
+        assert n.value == 0
+
+    for kw, word in CACHES + POOLS:
+        both(cache(lva, **kw), batch(lva), spec(lva), 0, word)
+    for kw, word in BATCHES:
+        both(cache(lva), batch(lva, **kw), spec(lva), 0, word)
+    for kw, word in [(dict(heads=0), "heads"), (dict(heads=12), "heads"), (dict(heads=1 << 17), "heads"), (dict(scale=float("nan")), "scale"), (dict(scale=float("inf")), "scale"),
+                     (dict(sinks=P + 2), "aligned")]:
+        both(cache(lva), batch(lva), spec(lva, **kw), 0, word)
+    both(cache(lva), batch(lva), spec(lva), lva.LV_Q4_0, "type")
+    both(cache(lva), batch(lva), None, 0, "spec is null")
+    both(cache(lva), batch(lva), spec(lva), 0, "ctx")
+    ok = cache(lva), batch(lva), spec(lva)
+    for out, ldo, q, ldq, kind, word in [(None, 4096, P, 4096, 0, "null"), (P, 4096, None, 4096, 0, "null"), (P, 4092, P, 4096, 0, "stride"), (P, 4096, P, 4092, 0, "stride"),
+                                         (P + 4, 4096, P, 4096, 0, "16 bytes"), (P, 4096, P + 2, 4096, 30, "16 bytes"), (P, 4100, P, 4096, 1, "16 bytes"),
+                                         (P, 4096, P, 4098, 0, "16 bytes")]:
+        refused(lva, call(None, out, ldo, q, ldq, kind, *ok, None, 0), word)
+    refused(lva, size(None, 0, *ok, None), "bytes is null")
+
+
+def test_cache_bytes(lva):
+    n = lva.C.c_uint64()
+    for kw, word in CACHES:
+        refused(lva, lva.hip().lv_paged_cache_bytes(cache(lva, **kw), n), word)
+        assert n.value == 0
+    refused(lva, lva.hip().lv_paged_cache_bytes(cache(lva), None), "bytes is null")
+    for kind in (ref.F16, ref.BF16, ref.Q8, ref.Q4):
+        for dim in (32, 64, 128, 256):
+            for page in (16, 64, 1024):
+                pool = ref.Pool(kind, 3, dim, page, 2)
+                assert lva.paged_cache_bytes(cache(lva, data=None, type=kind, kv_heads=3, dim=dim, page=page, pages=2)) == pool.bytes.nbytes
+    # beyond 32 bits
+    assert lva.paged_cache_bytes(cache(lva, pages=1 << 20, kv_heads=64)) == (1 << 20) * 64 * 2 * 16 * 256
+
+
+def test_rotate_refusals(lva):
+    call = lva.hip().lv_kernel_rotate
+
+    def one(word, out=P, ldo=512, x=P, ldx=512, kind=0, positions=P, tokens=3, heads=4, dim=128, rot=128, base=1e4, sections=(0, 0, 0), flags=0):
+        refused(lva, call(None, out, ldo, x, ldx, kind, positions, tokens, heads, dim, lva.RotateSpec(rot, base, sections, flags)), word)
+
+    one("type", kind=2)
+    for dim in (0, 12, 520):
+        one("dim", dim=dim, rot=0)
+    one("heads", heads=0)
+    one("heads", heads=1 << 17)
+    one("tokens", tokens=(1 << 24) + 1)
+    one("rot_dims", rot=127)
+    one("rot_dims", rot=130)
+    one("flags", flags=4)
+    for base in (0.0, -1.0, float("nan"), float("inf")):
+        one("rot_base", base=base)
+    one("sections", sections=(10, 20, 30))
+    one("sections", sections=(0xFFFFFFFF, 65, 0))
+    one("null", out=None)
+    one("null", x=None)
+    one("null", positions=None)
+    one("stride", ldx=508)
+    one("stride", ldo=508)
+    one("16 bytes", out=P + 4)
+    one("16 bytes", x=P + 8)
+    one("16 bytes", ldx=514)
+    one("16 bytes", ldo=516, kind=30)
+    one("4 bytes", positions=P + 2)
+    one("another stride", ldo=516)
+    one("ctx")
+    refused(lva, call(None, P, 512, P, 512, 0, P, 3, 4, 128, None), "spec is null")
+
+
+def test_verify_refusals(lva):
+    call, size = lva.hip().lv_kernel_verify_drafts, lva.hip().lv_verify_drafts_workspace
+    n = lva.C.c_uint64(7)
+
+    def drafts(**kw):
+        b = dict(seqs=2, drafts=4, vocab=1000, target=P, ld_target=1000, draft=P, ld_draft=1000, tokens=P, counts=P, uniforms=P)
+        b.update(kw)
+        return lva.DraftBatch(*b.values())
+
+    for kw, word in [(dict(seqs=70000), "sequences"), (dict(drafts=0), "drafts"), (dict(drafts=65), "drafts"), (dict(vocab=0), "vocab"), (dict(vocab=(1 << 24) + 1), "vocab"),
+                     (dict(ld_target=999), "stride"), (dict(ld_draft=999), "stride"), (dict(target=None), "null"), (dict(tokens=None), "null"), (dict(uniforms=None), "null"),
+                     (dict(target=P + 2), "aligned"), (dict(draft=P + 1), "aligned"), (dict(counts=P + 2), "aligned")]:
+        refused(lva, call(None, P, P, drafts(**kw), P, 1 << 20), word)
+        refused(lva, size(None, drafts(**kw), n), word)
+        assert n.value == 0
+    refused(lva, call(None, P, P, None, P, 1 << 20), "batch is null")
+    refused(lva, call(None, P, P, drafts(draft=None, ld_draft=0, counts=None), P, 1 << 20), "ctx")
+    refused(lva, size(None, drafts(), None), "bytes is null")
+    refused(lva, size(None, drafts(), n), "ctx")
+    refused(lva, lva.hip().lv_ctx_stream(None, None), "null")
+
+
+# ---- the arithmetic of lv_paged_plan.h, compiled for the host --------------------------------------------------------------------
+SOURCE = r"""
+#include "lv_paged_plan.h"
+#include <cstdio>
+#include <iostream>
+#include <string>
+#include <vector>
+int main()
+{
+    for (std::string what; std::cin >> what;) {
+        if (what == "row") {
+            lv_paged_cache c{};
+            uint32_t page, head, which, at;
+            std::cin >> c.type >> c.kv_heads >> c.dim >> c.page >> c.pages >> page >> head >> which >> at;
+            const lv::PagedView v = lv::paged_view(c);
+            printf("%llu %llu %u\n", (unsigned long long)lv::paged_codes(v, page, head, which, at), (unsigned long long)lv::paged_scales(v, page, head, which, at), v.block);
+        } else if (what == "page") {
+            lv_paged_cache c{};
+            uint32_t n, position;
+            c.kv_heads = 1, c.dim = 32, c.type = LV_F16;
+            std::cin >> c.page >> c.pages >> position >> n;
+            std::vector<uint32_t> row(n);
+            for (auto &x : row) std::cin >> x;
+            printf("%u\n", lv::paged_page(lv::paged_view(c), row.data(), n, position));
+        } else if (what == "seq") {
+            uint32_t start, end, len, tokens, positions;
+            std::cin >> start >> end >> len >> tokens >> positions;
+            const lv::PagedSeq s = lv::paged_seq(start, end, len, tokens, positions);
+            printf("%u %u %d %u\n", s.row0, s.rows, s.pos0, s.keys);
+        } else if (what == "first") {
+            uint32_t p, w, c;
+            std::cin >> p >> w >> c;
+            printf("%u\n", lv::paged_first_key(p, w, c));
+        } else if (what == "deal") {
+            lv::PagedDeal d{};
+            std::cin >> d.seqs >> d.group >> d.tile >> d.kv_heads >> d.window >> d.chunk >> d.positions >> d.target;
+            std::vector<uint32_t> lens(d.seqs), news(d.seqs);
+            for (uint32_t b = 0; b < d.seqs; b++) std::cin >> lens[b] >> news[b], d.tokens += news[b];
+            float all = 0;
+            uint32_t row = 0;
+            std::vector<lv::PagedSeq> s;
+            for (uint32_t b = 0; b < d.seqs; b++) {
+                s.push_back(lv::paged_seq(row, row + news[b], lens[b], d.tokens, d.positions));
+                row += news[b];
+                all += (float)lv::paged_tiles(d, s[b]) * (float)lv::paged_steps(d, s[b]);
+            }
+            const uint32_t run = lv::paged_run(d, all);
+            uint64_t items = 0;
+            // every key that a tile's rows see has to lie in its parts
+            uint32_t missed = 0, cut = 0;
+            for (const auto &x : s) {
+                const uint32_t steps = lv::paged_steps(d, x), parts = lv::paged_parts(steps, run), tiles = lv::paged_tiles(d, x);
+                items += (uint64_t)tiles * parts;
+                cut += parts > 1;
+                for (uint32_t t = 0; t < tiles; t++) {
+                    const uint32_t rows = x.rows * d.group, last = std::min((t + 1) * d.tile, rows) - 1;
+                    const int32_t p0 = x.pos0 + (int32_t)(t * d.tile / d.group), p1 = x.pos0 + (int32_t)(last / d.group);
+                    if (p1 < 0) continue;
+                    const uint32_t lo = p0 >= 0 ? lv::paged_first_key(p0, d.window, d.chunk) : 0, hi = std::min((uint32_t)p1 + 1, x.keys), base = lo & ~31u;
+                    if (hi > base && (uint64_t)parts * run * lv::kPagedStep < hi - base) missed++;
+                }
+            }
+            printf("%u %llu %llu %u %u\n", run, (unsigned long long)items, (unsigned long long)lv::paged_items(d), missed, cut);
+        }
+    }
+}
+"""
+
+
+@pytest.fixture(scope="module")
+def ask(tmp_path_factory):
+    d = tmp_path_factory.mktemp("plan")
+    (d / "main.cpp").write_text(SOURCE.replace("#include <cstdio>", "#include <algorithm>\n#include <cstdio>"))
+    subprocess.run(["g++", "-std=c++17", "-O1", "-Wall", "-Werror", "-I", CSRC, str(d / "main.cpp"), "-o", str(d / "main")], check=True)
+
+    def go(lines):
+        text = "\n".join(" ".join(map(str, q)) for q in lines)
+        out = subprocess.run([str(d / "main")], input=text, capture_output=True, text=True, check=True).stdout
+        return [tuple(map(int, line.split())) for line in out.splitlines()]
+    return go
+
+
+@pytest.mark.parametrize("kind", [ref.F16, ref.BF16, ref.Q8, ref.Q4], ids=lambda k: ref.NAMES[k])
+@pytest.mark.parametrize("dim,page", [(32, 16), (128, 32), (256, 1024)])
+def test_layout(ask, kind, dim, page):
+    pool = ref.Pool(kind, 3, dim, page, 4)
+    where = [(p, h, w, t) for p in (0, 3) for h in (0, 2) for w in (0, 1) for t in (0, 1, page - 1)]
+    base = pool.bytes.ctypes.data
+    for (p, h, w, t), (codes, scales, block) in zip(where, ask([("row", kind, 3, dim, page, 4, *x) for x in where])):
+        c, s = pool.row(p, h, w, t)
+        assert block == pool.block and codes == c.ctypes.data - base and codes % 16 == 0 or kind == ref.Q4 and dim == 32
+        if s.size:
+            assert scales == s.ctypes.data - base
+    # offsets beyond 32 bits
+    (codes, _, _), = ask([("row", kind, 64, dim, page, 1 << 20, (1 << 20) - 1, 63, 1, page - 1)])
+    assert codes == ((1 << 20) * 64 - 1) * pool.block + pool.half + (page - 1) * pool.code_row
+
+
+def test_pages_that_are_not_there(ask):
+    row = [2, 9, 10, 0xFFFFFFFF, 0]
+    q = [("page", 16, 10, p, len(row), *row) for p in (0, 15, 16, 31, 32, 48, 64, 79, 80, 1 << 30, 0xFFFFFFFF)]
+    assert [a for a, in ask(q)] == [2, 2, 9, 9] + [ref.NO_PAGE] * 2 + [0, 0] + [ref.NO_PAGE] * 3
+
+
+def test_rows_of_a_sequence(ask):
+    N = 1 << 30
+    got = ask([("seq", 3, 8, 20, 100, 4096), ("seq", 3, 3, 20, 100, 4096), ("seq", 8, 3, 20, 100, 4096), ("seq", 0, 5, 3, 100, 4096), ("seq", 0, 5, 0, 100, 4096),
+               ("seq", 0, 200, 300, 100, 4096), ("seq", 150, 200, 300, 100, 4096), ("seq", 0, 5, 5000, 100, 4096), ("seq", 0, 1, 0xFFFFFFFF, 100, N), ("seq", 0, 0xFFFFFFFF, 7, 100, N)])
+    assert got == [(3, 5, 15, 20), (3, 0, 20, 20), (8, 0, 20, 20), (0, 5, -2, 3), (0, 5, -5, 0),
+                   (0, 100, 100, 300), (150, 0, 250, 300), (0, 5, 4995, 4096), (0, 1, N - 1, N), (0, 100, 7 - N, 7)]
+
+
+def test_first_key(ask):
+    q = [(p, w, c) for p in (0, 1, 6, 7, 8, 99, N_BIG) for w in (0, 1, 7, 8, 200) for c in (0, 1, 7, 10, 1000)]
+    for (p, w, c), (got,) in zip(q, ask([("first", *x) for x in q])):
+        assert got == max(0, p - w + 1 if w else 0, p - p % c if c else 0), (p, w, c)
+
+
+N_BIG = (1 << 30) - 1
+
+
+def test_every_key_is_dealt(ask):
+    """no tile's keys lie outside its parts, and the launch's workgroups are enough for all items, for any mix of lengths"""
+    rng = np.random.default_rng(5)
+    qs = []
+    for n in range(400):
+        seqs = int(rng.integers(1, 200))
+        top = int(10 ** rng.uniform(0, 5.3))
+        new = np.where(rng.random(seqs) < 0.7, 1, rng.integers(0, int(10 ** rng.uniform(0, 3)) + 1, seqs))
+        lens = np.maximum(rng.integers(0, top + 1, seqs), np.where(rng.random(seqs) < 0.9, new, 0))
+        if n % 5 == 0:
+            lens[0] = 200000
+        qs.append(("deal", seqs, int(rng.integers(1, 9)), int(rng.choice([16, 32, 64, 128])), int(rng.choice([1, 4, 8, 40])), int(rng.choice([0, 0, 7, 512])),
+                   int(rng.choice([0, 0, 10, 1000])), 1 << 20, int(rng.choice([0, 256, 1024])), *np.stack([lens, new], 1).reshape(-1).tolist()))
+    cut = 0
+    for q, (run, items, room, missed, c) in zip(qs, ask(qs)):
+        assert missed == 0 and items <= room, q[:9]
+        assert q[8] or c == 0
+        cut += c > 0
+    assert cut > 30      # calls in which something is cut
+
+
+def test_one_long_sequence_is_cut_and_equal_ones_are_not(ask):
+    one = ask([("deal", 1, 4, 16, 8, 0, 0, 1 << 20, 1024, 131072, 1)])[0]
+    assert one[1] >= 100 and one[4] == 1
+    many = ask([("deal", 128, 4, 16, 8, 0, 0, 1 << 20, 1024, *([4096, 1] * 128))])[0]
+    assert many[1] <= 2 * 128
+    mixed = ask([("deal", 64, 4, 16, 8, 0, 0, 1 << 20, 1024, 131072, 1, *([100, 1] * 63))])[0]
+    assert mixed[1] >= 100 + 63 and mixed[4] == 1
