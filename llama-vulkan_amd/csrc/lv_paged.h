@@ -80,7 +80,7 @@ __device__ __forceinline__ float paged_all_steps(const PagedAttnArgs &a, int lan
 template <bool BY_ROW> __device__ __forceinline__ PagedItem paged_locate(const PagedAttnArgs &a, uint32_t which, int lane, uint32_t sub = 0)
 {
     PagedItem it{};
-    it.run = paged_run(a.deal, a.deal.target ? paged_all_steps(a, lane) : 0.f);
+    it.run = __builtin_amdgcn_readfirstlane(paged_run(a.deal, a.deal.target ? paged_all_steps(a, lane) : 0.f));
     uint32_t before = 0;
     for (uint32_t b0 = 0; b0 < a.deal.seqs; b0 += 64) {
         PagedSeq s{};
@@ -116,9 +116,26 @@ template <bool BY_ROW> __device__ __forceinline__ PagedItem paged_locate(const P
 }
 
 // ---- elements ----------------------------------------------------------------------------------------------------------------------
-__device__ __forceinline__ float pg_bf16(uint32_t h) { return __uint_as_float(h << 16); }
 __device__ __forceinline__ float pg_exp2(float x) { return __builtin_amdgcn_exp2f(x); }      // 1 ulp; 0 below 2^-126
 
+// eight 16-bit numbers of one kind
+template <bool BF> __device__ __forceinline__ void pg_unpack8(uint4 u, float (&x)[8])
+{
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        x[2 * i] = BF ? __uint_as_float(w[i] << 16) : half_bits_to_float((uint16_t)w[i]);
+        x[2 * i + 1] = BF ? __uint_as_float(w[i] & 0xffff0000u) : half_bits_to_float((uint16_t)(w[i] >> 16));
+    }
+}
+__device__ __forceinline__ uint32_t pg_bits(float x, bool half) { return half ? (uint32_t)float_to_half_bits(x) : (uint32_t)__builtin_bit_cast(uint16_t, (__bf16)x); }
+template <bool BF> __device__ __forceinline__ uint4 pg_pack8(const float (&x)[8])
+{
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) w[i] = pg_bits(x[2 * i], !BF) | (pg_bits(x[2 * i + 1], !BF) << 16);
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
 // eight elements of `type` from `at` on
 __device__ __forceinline__ void pg_load8(const void *p, uint32_t type, uint64_t at, float (&x)[8])
 {
@@ -129,16 +146,8 @@ __device__ __forceinline__ void pg_load8(const void *p, uint32_t type, uint64_t 
         return;
     }
     const uint4 u = *reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(p) + at);
-    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-        x[2 * i] = type == LV_F16 ? half_bits_to_float((uint16_t)w[i]) : pg_bf16(w[i] & 0xffffu);
-        x[2 * i + 1] = type == LV_F16 ? half_bits_to_float((uint16_t)(w[i] >> 16)) : __uint_as_float(w[i] & 0xffff0000u);
-    }
-}
-__device__ __forceinline__ uint32_t pg_bits(float x, uint32_t type)
-{
-    return type == LV_F16 ? (uint32_t)float_to_half_bits(x) : (uint32_t)__builtin_bit_cast(uint16_t, (__bf16)x);
+    if (type == LV_F16) pg_unpack8<false>(u, x);
+    else pg_unpack8<true>(u, x);
 }
 __device__ __forceinline__ void pg_store8(void *p, uint32_t type, uint64_t at, const float (&x)[8])
 {
@@ -148,10 +157,37 @@ __device__ __forceinline__ void pg_store8(void *p, uint32_t type, uint64_t at, c
         f[1] = make_float4(x[4], x[5], x[6], x[7]);
         return;
     }
-    uint32_t w[4];
+    *reinterpret_cast<uint4 *>(static_cast<uint16_t *>(p) + at) = type == LV_F16 ? pg_pack8<false>(x) : pg_pack8<true>(x);
+}
+// N times eight elements, eight of them every `step`: all loads before the first use
+template <int N> __device__ __forceinline__ void pg_load_row(const void *p, uint32_t type, uint64_t at, uint32_t step, float (&x)[N][8])
+{
+    uint4 u[N], v[N];
+    if (type == LV_F32) {
+        const uint4 *f = reinterpret_cast<const uint4 *>(static_cast<const float *>(p) + at);
 #pragma unroll
-    for (int i = 0; i < 4; i++) w[i] = pg_bits(x[2 * i], type) | (pg_bits(x[2 * i + 1], type) << 16);
-    *reinterpret_cast<uint4 *>(static_cast<uint16_t *>(p) + at) = make_uint4(w[0], w[1], w[2], w[3]);
+        for (int n = 0; n < N; n++) {
+            u[n] = f[n * (step / 4)];
+            v[n] = f[n * (step / 4) + 1];
+        }
+#pragma unroll
+        for (int n = 0; n < N; n++) {
+            const uint32_t w[8] = {u[n].x, u[n].y, u[n].z, u[n].w, v[n].x, v[n].y, v[n].z, v[n].w};
+#pragma unroll
+            for (int e = 0; e < 8; e++) x[n][e] = __uint_as_float(w[e]);
+        }
+        return;
+    }
+    const uint4 *h = reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(p) + at);
+#pragma unroll
+    for (int n = 0; n < N; n++) u[n] = h[n * (step / 8)];
+    if (type == LV_F16) {
+#pragma unroll
+        for (int n = 0; n < N; n++) pg_unpack8<false>(u[n], x[n]);
+    } else {
+#pragma unroll
+        for (int n = 0; n < N; n++) pg_unpack8<true>(u[n], x[n]);
+    }
 }
 
 // codes to fp16: the byte under 0x64 is 1024 + byte
@@ -192,6 +228,25 @@ template <bool BF, int N, class Frag> __device__ __forceinline__ void pg_cut(flo
     }
 }
 
+// bits where one of two 16-bit numbers is not finite
+template <bool BF> __device__ __forceinline__ uint32_t pg_special(uint32_t w)
+{
+    return BF ? ((w & 0x7f807f80u) + 0x00800080u) & 0x80008000u : ((w & 0x7c007c00u) + 0x04000400u) & 0x80008000u;
+}
+// kind 0: the finite ones of eight numbers, 0 in place of others; 1, 2, 3: a one in place of each NaN, inf, -inf, 0 of others
+template <bool BF> __device__ __forceinline__ typename PgFrag<BF>::type pg_only(typename PgFrag<BF>::type f, int kind)
+{
+    pg_s8 s = __builtin_bit_cast(pg_s8, f);
+    constexpr int EX = BF ? 0x7f80 : 0x7c00;
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+        const int h = (uint16_t)s[e], size = h & 0x7fff;
+        const bool finite = size < EX, yes = kind == 1 ? size > EX : h == (kind == 2 ? EX : EX | 0x8000);
+        s[e] = (short)(kind == 0 ? (finite ? h : 0) : yes ? (BF ? 0x3f80 : 0x3c00) : 0);
+    }
+    return __builtin_bit_cast(typename PgFrag<BF>::type, s);
+}
+
 // the columns of a 4 x 16 tile of 16-bit elements; each of 16 lanes names the 8 bytes at row lane / 4, columns 4 (lane % 4) ..
 __device__ __forceinline__ pg_s4 pg_read_columns(const uint8_t *p)
 {
@@ -207,15 +262,23 @@ __device__ __forceinline__ pg_s4 pg_read_columns(const uint8_t *p)
 // NQ: pieces of a query, 1, or with 32-bit queries 2 (fp16 rows: 22 bits) or 3 (bf16 rows: 24 bits); the weights have as many, 2 of bf16 at least.  Rows of
 // codes: keys enter as exact integers, a block's sum is scaled in fp32.  Values are scaled in fp16 (a rounding of 2^-11 of each, beside the 16-bit result's own); with
 // 32-bit queries they enter as two fp16 pieces, which hold them exactly: 19 bits at most, the last of them 2^-24 or more, as the scale's is.
+// waves a SIMD that the registers are cut for: as many as leave none in memory
+constexpr int paged_rows_waves(int D, int CT, int NQ, int QT)
+{
+    if (D == 256) return 1;
+    if (D == 128) return QT == 1 && NQ == 1 && CT >= kPgQ8 ? 3 : 2;
+    return NQ > 1 && QT == 2 ? 2 : 3;
+}
+
 template <int D, int CT, int NQ, int QT>
-__global__ __launch_bounds__(256) void paged_rows_kernel(PagedAttnArgs a)
+__global__ __launch_bounds__(256, paged_rows_waves(D, CT, NQ, QT)) void paged_rows_kernel(PagedAttnArgs a)
 {
     constexpr bool BF = CT == kPgBf16, BLOCKS = CT == kPgQ8 || CT == kPgQ4, EXACT = NQ > 1;
-    constexpr int KS = D / 32, DT = D / 16, CH = D / 8, SW = CH < 16 ? CH - 1 : 15, NP = BF && NQ == 1 ? 2 : NQ, TILE = 16 * QT;
+    constexpr int KS = D / 32, DT = D / 16, CH = D / 8, ROW = 2 * D + 16, NP = BF && NQ == 1 ? 2 : NQ, TILE = 16 * QT;
     constexpr float kLift = BF ? 0.f : 12.f;
     constexpr int MERGE = D + 4;                      // floats of a row of results in LDS
     typedef typename PgFrag<BF>::type Frag;
-    constexpr int PLANES = BLOCKS && EXACT ? 2 : 1, VALUES = 32 * D * 2 * PLANES;      // bytes of a wave's 32 rows of values
+    constexpr int PLANES = BLOCKS && EXACT ? 2 : 1, VALUES = 32 * ROW * PLANES;      // bytes of a wave's 32 rows of values; 16 more a row put the 16 rows of a column read on all banks evenly
     __shared__ __attribute__((aligned(128))) uint8_t lds[4 * VALUES > 4 * 16 * MERGE * 4 ? 4 * VALUES : 4 * 16 * MERGE * 4];      // at the end 16 rows of results of each wave
     __shared__ float ml[4][TILE][2];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l16 = lane & 15, g4 = lane >> 4;
@@ -228,34 +291,36 @@ __global__ __launch_bounds__(256) void paged_rows_kernel(PagedAttnArgs a)
     // this lane's rows
     Frag q[QT][KS][NQ];
     float factor[QT];
-    int32_t lo[QT], hi[QT];
+    uint32_t lo[QT], span[QT];      // the keys it sees: lo .. lo + span - 1
 #pragma unroll
     for (int i = 0; i < QT; i++) {
         const uint32_t r = r0 + i * 16 + l16;
         const bool mine = r < rows;
         const uint32_t t = mine ? r / group : 0, h = head * group + (mine ? r - t * group : 0);
         const int32_t p = it.s.pos0 + (int32_t)t;
-        hi[i] = mine ? p : -1;
-        lo[i] = p >= 0 ? (int32_t)paged_first_key((uint32_t)p, a.deal.window, a.deal.chunk) : 0;
-        float x[KS][8], top = 0.f;
+        lo[i] = p >= 0 ? paged_first_key((uint32_t)p, a.deal.window, a.deal.chunk) : 0;
+        const uint32_t end = p >= 0 ? min((uint32_t)p + 1, it.s.keys) : 0;
+        span[i] = mine && end > lo[i] ? end - lo[i] : 0;
+        float z[KS][8], top = 0.f;
         const uint64_t at = (uint64_t)(it.s.row0 + t) * a.ldq + (uint64_t)h * D;
+        if constexpr (CT == kPgQ4) {      // byte 4 g + j of a block holds elements 4 g + j and 16 + 4 g + j
+            float u[2 * KS][8];
+            pg_load_row<2 * KS>(a.q, a.type, at + (g4 / 2) * 8, 16, u);
 #pragma unroll
-        for (int k = 0; k < KS; k++) {
-            if constexpr (CT == kPgQ4) {      // byte 4 g + j of a block holds elements 4 g + j and 16 + 4 g + j
-                float u[8], v[8];
-                pg_load8(a.q, a.type, at + k * 32 + (g4 / 2) * 8, u);
-                pg_load8(a.q, a.type, at + k * 32 + 16 + (g4 / 2) * 8, v);
+            for (int k = 0; k < KS; k++)
 #pragma unroll
                 for (int e = 0; e < 4; e++) {
-                    x[k][e] = g4 & 1 ? u[4 + e] : u[e];
-                    x[k][4 + e] = g4 & 1 ? v[4 + e] : v[e];
+                    const float a0 = u[2 * k][e], a1 = u[2 * k][4 + e], b0 = u[2 * k + 1][e], b1 = u[2 * k + 1][4 + e];
+                    z[k][e] = g4 & 1 ? a1 : a0;
+                    z[k][4 + e] = g4 & 1 ? b1 : b0;
                 }
-            } else {
-                pg_load8(a.q, a.type, at + k * 32 + g4 * 8, x[k]);
-            }
-#pragma unroll
-            for (int e = 0; e < 8; e++) top = fmaxf(top, fabsf(x[k][e]));
+        } else {
+            pg_load_row<KS>(a.q, a.type, at + g4 * 8, 32, z);
         }
+#pragma unroll
+        for (int k = 0; k < KS; k++)
+#pragma unroll
+            for (int e = 0; e < 8; e++) top = fmaxf(top, fabsf(z[k][e]));
         top = fmaxf(top, __shfl_xor(top, 16, 64));
         top = fmaxf(top, __shfl_xor(top, 32, 64));
         // a power of two brings the row's largest element to 2^10 .. 2^11: no overflow, and small pieces are no subnormals
@@ -266,7 +331,7 @@ __global__ __launch_bounds__(256) void paged_rows_kernel(PagedAttnArgs a)
 #pragma unroll
         for (int k = 0; k < KS; k++)
 #pragma unroll
-            for (int e = 0; e < 8; e++) pg_cut<BF, NQ>(mine ? x[k][e] * down : 0.f, e, q[i][k]);
+            for (int e = 0; e < 8; e++) pg_cut<BF, NQ>(mine ? z[k][e] * down : 0.f, e, q[i][k]);
     }
     // keys that any row sees, and those that all rows see
     const uint32_t last_row = min(r0 + TILE, rows) - 1;
@@ -289,42 +354,50 @@ __global__ __launch_bounds__(256) void paged_rows_kernel(PagedAttnArgs a)
         uint4 v4[CT <= kPgBf16 ? D / 16 : CT == kPgQ8 ? D / 32 : 1];        // 16 bytes of a row
         uint2 v2[CT == kPgQ4 ? D / 32 : 1];                                 // 8 bytes: half a block's
         uint16_t vd[BLOCKS ? D / 32 : 1];
-        bool ok[2];                                                         // 16 keys each: is there a page?
     };
     // row of 32 and unit of the row that this lane brings with its i-th load of values
     constexpr int UNITS = CT <= kPgBf16 ? CH : D / 16, LOADS = 32 * UNITS / 64;
-    auto row_of = [&](int i) { return (i * 64 + lane) / UNITS; };
-    auto unit_of = [&](int i) { return (i * 64 + lane) % UNITS; };
-    auto load = [&](Turn &x, uint32_t t) {
-        const uint32_t kb = base + t * 32;
-        const uint8_t *pk[2], *pv[2], *pks[2], *pvs[2];
+    // (addresses are made anew in every turn, from a lane number that the compiler cannot see through: kept, they would take a hundred registers)
+    int ln = lane;
+    auto row_of = [&](int i) { return (i * 64 + ln) / UNITS; };
+    auto unit_of = [&](int i) { return (i * 64 + ln) % UNITS; };
+    // where 16 keys' codes lie (of keys; of values and scales at the same distances in every block), null without a page
+    Turn x;
+    auto place = [&](uint32_t t, int kt, uint32_t &in) {
+        const uint32_t at = base + t * 32 + 16 * kt, page = __builtin_amdgcn_readfirstlane(paged_page(a.c, table, a.table_ld, at));
+        in = at & (psize - 1);
+        return page;
+    };
+    auto block_of = [&](uint32_t page) { return a.c.data + ((uint64_t)(page != kNoPage ? page : 0) * a.c.kv_heads + head) * a.c.block; };
+    const uint32_t scales_at = a.c.code_row << a.c.shift;
+    auto load_keys = [&](uint32_t page0, uint32_t page1, uint32_t in0, uint32_t in1) {
 #pragma unroll
         for (int kt = 0; kt < 2; kt++) {
-            const uint32_t at = kb + 16 * kt, page = paged_page(a.c, table, a.table_ld, at), in = at & (psize - 1);
-            x.ok[kt] = page != kNoPage;
-            const uint8_t *block = a.c.data + ((uint64_t)(x.ok[kt] ? page : 0) * a.c.kv_heads + head) * a.c.block;
-            pk[kt] = block + in * a.c.code_row;
-            pv[kt] = pk[kt] + a.c.half;
-            pks[kt] = block + (a.c.code_row << a.c.shift) + in * a.c.scale_row;
-            pvs[kt] = pks[kt] + a.c.half;
-        }
-#pragma unroll
-        for (int kt = 0; kt < 2; kt++)
+            const uint8_t *block = block_of(kt ? page1 : page0);
+            const uint32_t in = kt ? in1 : in0;
+            const uint8_t *pk = block + in * a.c.code_row, *ps = block + scales_at + in * a.c.scale_row;
 #pragma unroll
             for (int k = 0; k < KS; k++) {
-                if constexpr (CT <= kPgBf16) x.k4[kt][k] = *reinterpret_cast<const uint4 *>(pk[kt] + (uint32_t)(l16 * (2 * D) + k * 64 + g4 * 16));
-                else if constexpr (CT == kPgQ8) x.k2[kt][k] = *reinterpret_cast<const uint2 *>(pk[kt] + (uint32_t)(l16 * D + k * 32 + g4 * 8));
-                else x.k1[kt][k] = *reinterpret_cast<const uint32_t *>(pk[kt] + (uint32_t)(l16 * (D / 2) + k * 16 + g4 * 4));
-                if constexpr (BLOCKS) x.ks[kt][k] = *reinterpret_cast<const uint2 *>(pks[kt] + (uint32_t)(g4 * (D / 4) + k * 8));
+                if constexpr (CT <= kPgBf16) x.k4[kt][k] = *reinterpret_cast<const uint4 *>(pk + (uint32_t)((ln & 15) * (2 * D) + k * 64 + (ln >> 4) * 16));
+                else if constexpr (CT == kPgQ8) x.k2[kt][k] = *reinterpret_cast<const uint2 *>(pk + (uint32_t)((ln & 15) * D + k * 32 + (ln >> 4) * 8));
+                else x.k1[kt][k] = *reinterpret_cast<const uint32_t *>(pk + (uint32_t)((ln & 15) * (D / 2) + k * 16 + (ln >> 4) * 4));
+                if constexpr (BLOCKS) x.ks[kt][k] = *reinterpret_cast<const uint2 *>(ps + (uint32_t)((ln >> 4) * (D / 4) + k * 8));
             }
+        }
+    };
+    auto load_values = [&](uint32_t page0, uint32_t page1, uint32_t in0, uint32_t in1) {
+        const uint8_t *block0 = block_of(page0) + a.c.half, *block1 = block_of(page1) + a.c.half;
+        const uint8_t *pv0 = block0 + in0 * a.c.code_row, *pv1 = block1 + in1 * a.c.code_row;
+        const uint8_t *ps0 = block0 + scales_at + in0 * a.c.scale_row, *ps1 = block1 + scales_at + in1 * a.c.scale_row;
 #pragma unroll
         for (int i = 0; i < LOADS; i++) {
             const int row = row_of(i), u = unit_of(i);
-            const uint8_t *p = row < 16 ? pv[0] : pv[1];
+            const bool second = 64 / UNITS <= 16 ? i * (64 / UNITS) >= 16 : row >= 16;      // of 16 keys; where a load covers no more, the same in all lanes
+            const uint8_t *p = second ? pv1 : pv0, *ps = second ? ps1 : ps0;
             if constexpr (CT <= kPgBf16) x.v4[i] = *reinterpret_cast<const uint4 *>(p + (uint32_t)((row & 15) * (2 * D) + u * 16));
             else if constexpr (CT == kPgQ8) x.v4[i] = *reinterpret_cast<const uint4 *>(p + (uint32_t)((row & 15) * D + u * 16));
             else x.v2[i] = *reinterpret_cast<const uint2 *>(p + (uint32_t)((row & 15) * (D / 2) + u * 8));
-            if constexpr (BLOCKS) x.vd[i] = *reinterpret_cast<const uint16_t *>((row < 16 ? pvs[0] : pvs[1]) + (uint32_t)((row & 15) * (D / 16) + u / 2 * 2));
+            if constexpr (BLOCKS) x.vd[i] = *reinterpret_cast<const uint16_t *>(ps + (uint32_t)((row & 15) * (D / 16) + u / 2 * 2));
         }
     };
 
@@ -338,24 +411,59 @@ __global__ __launch_bounds__(256) void paged_rows_kernel(PagedAttnArgs a)
         for (int d = 0; d < DT; d++) o[d][i] = pg_f4{0.f, 0.f, 0.f, 0.f};
     }
     // eight elements into chunk `ch` of a row of values in LDS
-    auto put = [&](int row, int ch, uint4 w, int plane = 0) { *reinterpret_cast<uint4 *>(mine + plane * (32 * D * 2) + row * (2 * D) + ((ch ^ (row & SW)) * 16)) = w; };
-    // first operand of O^T for dimensions 16 d ..: dimension l16, keys 4 g .. + 3 and 16 + 4 g .. + 3
+    auto put = [&](int row, int ch, uint4 w, int plane = 0) { *reinterpret_cast<uint4 *>(mine + plane * (32 * ROW) + row * ROW + ch * 16) = w; };
+    // first operand of O^T for dimensions 16 d ..: dimension (ln & 15), keys 4 g .. + 3 and 16 + 4 g .. + 3
     auto values = [&](int d, int plane = 0) {
-        const int row = 4 * g4 + l16 / 4, c = 16 * d + 4 * (l16 & 3);
-        const int off = (c % 8) * 2 + plane * (32 * D * 2);
-        const pg_s4 u = pg_read_columns(mine + row * (2 * D) + (((c / 8) ^ (row & SW)) * 16) + off);
-        const pg_s4 v = pg_read_columns(mine + (row + 16) * (2 * D) + (((c / 8) ^ ((row + 16) & SW)) * 16) + off);
+        const uint8_t *at = mine + (4 * (ln >> 4) + (ln & 15) / 4) * ROW + 8 * (ln & 3) + 32 * d + plane * (32 * ROW);
+        const pg_s4 u = pg_read_columns(at), v = pg_read_columns(at + 16 * ROW);
         return __builtin_bit_cast(Frag, pg_s8{u[0], u[1], u[2], u[3], v[0], v[1], v[2], v[3]});
     };
 
-    auto use = [&](Turn &x, uint32_t t) {
+    // does row i see key 16 kt + 4 g + r of a turn?
+    auto sees = [&](uint32_t kb, bool ok, int i, int kt, int r) { return kb + (kt * 16 + (ln >> 4) * 4 + r) - lo[i] < (ok ? span[i] : 0u); };
+    // Values that no row sees are made 0: a page's rows behind the sequence's end may hold anything, and 0 times that has to be 0.
+    auto clear = [&](uint32_t kb, bool ok0, bool ok1) {
+#pragma unroll
+        for (int i = 0; i < LOADS; i++) {
+            const int row = row_of(i);
+            const bool keep = kb + row - k_lo < ((row < 16 ? ok0 : ok1) ? k_hi - k_lo : 0u);
+            if constexpr (CT <= kPgBf16) {
+                if (!keep) x.v4[i] = make_uint4(0, 0, 0, 0);
+            } else {
+                if (!keep) x.vd[i] = 0;
+            }
+        }
+    };
+    auto any_special = [&]() {
+        uint32_t odd = 0;
+        if constexpr (CT <= kPgBf16) {
+#pragma unroll
+            for (int i = 0; i < LOADS; i++) odd |= pg_special<BF>(x.v4[i].x) | pg_special<BF>(x.v4[i].y) | pg_special<BF>(x.v4[i].z) | pg_special<BF>(x.v4[i].w);
+        }
+        return __any(odd != 0);
+    };
+    bool special = false;
+    const uint32_t t_first = s0 * 4 + wave;
+    uint32_t t = t_first, page0 = kNoPage, page1 = kNoPage;
+    if (t < t_end) {
+        uint32_t in0, in1;
+        page0 = place(t, 0, in0);
+        page1 = place(t, 1, in1);
+        load_keys(page0, page1, in0, in1);
+        load_values(page0, page1, in0, in1);
+    }
+    for (; t < t_end; t += 4) {
+        asm volatile("" : "+v"(ln));
         const uint32_t kb = base + t * 32;
-        const bool inside = kb >= k_lo && kb + 32 <= k_hi && x.ok[0] && x.ok[1];        // every key of the turn is some row's
+        const bool ok0 = page0 != kNoPage, ok1 = page1 != kNoPage;
+        const bool inside = kb >= k_lo && kb + 32 <= k_hi && ok0 && ok1;                // every key of the turn is some row's
         const bool edge = kb < all_lo || kb + 32 > all_hi || !inside;                   // some row does not see all of them
-        auto sees = [&](int i, int kt, int r) {
-            const int32_t p = (int32_t)(kb + kt * 16 + g4 * 4 + r);
-            return p >= lo[i] && p <= hi[i] && p < (int32_t)k_hi && x.ok[kt];
-        };
+        // the next turn's pages; its keys are asked for as soon as this turn's are used up, its values likewise
+        // (the last one asks for its own again, which are in the caches: a condition around the loads costs registers)
+        const uint32_t next = t + 4 < t_end ? t + 4 : t;
+        uint32_t in0, in1;
+        page0 = place(next, 0, in0);
+        page1 = place(next, 1, in1);
         pg_f4 sc[2][QT];
 #pragma unroll
         for (int kt = 0; kt < 2; kt++) {
@@ -395,16 +503,19 @@ __global__ __launch_bounds__(256) void paged_rows_kernel(PagedAttnArgs a)
                 }
             }
         }
+        load_keys(page0, page1, in0, in1);
         Frag p[QT][NP];
 #pragma unroll
         for (int i = 0; i < QT; i++) {
             float s[8], top = m[i];
 #pragma unroll
-            for (int e = 0; e < 8; e++) {
-                s[e] = sc[e / 4][i][e % 4] * factor[i];
-                if (edge && !sees(i, e / 4, e % 4)) s[e] = -INFINITY;
-                top = fmaxf(top, s[e]);
+            for (int e = 0; e < 8; e++) s[e] = sc[e / 4][i][e % 4] * factor[i];
+            if (edge) {
+#pragma unroll
+                for (int e = 0; e < 8; e++) s[e] = sees(kb, e < 4 ? ok0 : ok1, i, e / 4, e % 4) ? s[e] : -INFINITY;
             }
+#pragma unroll
+            for (int e = 0; e < 8; e++) top = fmaxf(top, s[e]);
             top = fmaxf(top, __shfl_xor(top, 16, 64));
             top = fmaxf(top, __shfl_xor(top, 32, 64));
             if (__any(top > m[i])) {
@@ -425,67 +536,13 @@ __global__ __launch_bounds__(256) void paged_rows_kernel(PagedAttnArgs a)
             }
             l[i] += sum;
         }
-        // Values that no row sees are made 0: a page's rows behind the sequence's end may hold anything, and 0 times that has to be 0.  Numbers that are not
-        // finite are taken out and added apart to the rows that see them: a weight that is 0, or a negative piece of one, would spread them or turn their sign.
-        if (!inside) {
+        if (!inside) clear(kb, ok0, ok1);
+        // Numbers that are not finite are left out here and added apart, behind the loop, to the rows that see them: a weight that is 0, or a negative piece of
+        // one, would spread them or turn their sign.
+        if (CT <= kPgBf16 && any_special()) {
+            special = true;
 #pragma unroll
-            for (int i = 0; i < LOADS; i++) {
-                const int row = row_of(i);
-                const bool keep = kb + row >= k_lo && kb + row < k_hi && (row < 16 ? x.ok[0] : x.ok[1]);
-                if constexpr (CT <= kPgBf16) {
-                    if (!keep) x.v4[i] = make_uint4(0, 0, 0, 0);
-                } else {
-                    if (!keep) x.vd[i] = 0;
-                }
-            }
-        }
-        if constexpr (CT <= kPgBf16) {
-            constexpr uint32_t EXP = BF ? 0x7f807f80u : 0x7c007c00u, ONE = BF ? 0x00800080u : 0x04000400u;
-            uint32_t odd = 0;
-#pragma unroll
-            for (int i = 0; i < LOADS; i++)
-                odd |= (((x.v4[i].x & EXP) + ONE) | ((x.v4[i].y & EXP) + ONE) | ((x.v4[i].z & EXP) + ONE) | ((x.v4[i].w & EXP) + ONE)) & 0x80008000u;
-            if (__any(odd != 0)) {
-                // 0: NaN, 1: inf, 2: -inf.  Counts of each among the keys a row sees, as a product of ones
-                for (int kind = 0; kind < 3; kind++) {
-                    auto count = [&](uint32_t w) {
-                        uint32_t out = 0;
-#pragma unroll
-                        for (int e = 0; e < 2; e++) {
-                            const uint32_t h = (w >> (16 * e)) & 0xffffu, ex = EXP & 0xffffu;
-                            const bool special = (h & ex) == ex, nan = special && (h & 0x7fffu) != ex;
-                            const bool yes = kind == 0 ? nan : special && !nan && (h >> 15) == (uint32_t)(kind - 1);
-                            out |= yes ? (BF ? 0x3f80u : 0x3c00u) << (16 * e) : 0u;
-                        }
-                        return out;
-                    };
-#pragma unroll
-                    for (int i = 0; i < LOADS; i++) put(row_of(i), unit_of(i), make_uint4(count(x.v4[i].x), count(x.v4[i].y), count(x.v4[i].z), count(x.v4[i].w)));
-                    const float add = kind == 0 ? __builtin_nanf("") : kind == 1 ? INFINITY : -INFINITY;
-#pragma unroll
-                    for (int i = 0; i < QT; i++) {
-                        Frag one;
-#pragma unroll
-                        for (int e = 0; e < 8; e++) {
-                            const float s = sees(i, e / 4, e % 4) ? 1.f : 0.f;
-                            if constexpr (BF) one[e] = (__bf16)s;
-                            else one[e] = (_Float16)s;
-                        }
-#pragma unroll
-                        for (int d = 0; d < DT; d++) {
-                            const pg_f4 n = pg_mfma<BF>(values(d), one, pg_f4{0.f, 0.f, 0.f, 0.f});
-#pragma unroll
-                            for (int r = 0; r < 4; r++) o[d][i][r] += n[r] > 0.f ? add : 0.f;
-                        }
-                    }
-                }
-                auto finite = [&](uint32_t w) {
-                    const uint32_t ex = EXP & 0xffffu;
-                    return (((w & ex) == ex) ? 0u : w & 0xffffu) | ((((w >> 16) & ex) == ex) ? 0u : w & 0xffff0000u);
-                };
-#pragma unroll
-                for (int i = 0; i < LOADS; i++) x.v4[i] = make_uint4(finite(x.v4[i].x), finite(x.v4[i].y), finite(x.v4[i].z), finite(x.v4[i].w));
-            }
+            for (int i = 0; i < (CT <= kPgBf16 ? LOADS : 0); i++) x.v4[i] = __builtin_bit_cast(uint4, pg_only<BF>(__builtin_bit_cast(Frag, x.v4[i]), 0));
         }
 #pragma unroll
         for (int i = 0; i < LOADS; i++) {
@@ -525,6 +582,7 @@ __global__ __launch_bounds__(256) void paged_rows_kernel(PagedAttnArgs a)
                 }
             }
         }
+        load_values(page0, page1, in0, in1);
 #pragma unroll
         for (int d = 0; d < DT; d++) {
             if constexpr (PLANES == 2) {      // the smaller pieces first; the product of both smaller ones is 2^-22 of the whole
@@ -538,17 +596,45 @@ __global__ __launch_bounds__(256) void paged_rows_kernel(PagedAttnArgs a)
 #pragma unroll
                 for (int n = NP - 1; n >= 0; n--) o[d][i] = pg_mfma<BF>(v, p[i][n], o[d][i]);
         }
-    };
+    }
 
-    uint32_t t = s0 * 4 + wave;
-    Turn x;
-    if (t < t_end) load(x, t);
-    while (t < t_end) {
-        Turn next = x;
-        if (t + 4 < t_end) load(next, t + 4);
-        use(x, t);
-        x = next;
-        t += 4;
+    if (CT <= kPgBf16 && special) {
+        for (t = t_first; t < t_end; t += 4) {
+            const uint32_t kb = base + t * 32;
+            uint32_t in0, in1;
+            page0 = place(t, 0, in0);
+            page1 = place(t, 1, in1);
+            const bool ok0 = page0 != kNoPage, ok1 = page1 != kNoPage;
+            load_values(page0, page1, in0, in1);
+            clear(kb, ok0, ok1);
+            if (!any_special()) continue;
+#pragma unroll
+            for (int i = 0; i < (CT <= kPgBf16 ? LOADS : 0); i++) put(row_of(i), unit_of(i), x.v4[i]);
+            // 1: NaN, 2: inf, 3: -inf.  Counts of each among the keys that a row sees, as a product of ones
+#pragma unroll 1
+            for (int kind = 1; kind <= 3; kind++) {
+                const float add = kind == 1 ? __builtin_nanf("") : kind == 2 ? INFINITY : -INFINITY;
+                Frag one[QT];
+#pragma unroll
+                for (int i = 0; i < QT; i++)
+#pragma unroll
+                    for (int e = 0; e < 8; e++) {
+                        const float w = sees(kb, e < 4 ? ok0 : ok1, i, e / 4, e % 4) ? 1.f : 0.f;
+                        if constexpr (BF) one[i][e] = (__bf16)w;
+                        else one[i][e] = (_Float16)w;
+                    }
+#pragma unroll
+                for (int d = 0; d < DT; d++) {
+                    const Frag v = pg_only<BF>(values(d), kind);
+#pragma unroll
+                    for (int i = 0; i < QT; i++) {
+                        const pg_f4 n = pg_mfma<BF>(v, one[i], pg_f4{0.f, 0.f, 0.f, 0.f});
+#pragma unroll
+                        for (int r = 0; r < 4; r++) o[d][i][r] += n[r] > 0.f ? add : 0.f;
+                    }
+                }
+            }
+        }
     }
 
     // the four waves' results put together, 16 rows at a time

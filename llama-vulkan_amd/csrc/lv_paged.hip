@@ -29,6 +29,7 @@ AttnPlan attn_plan(uint32_t units, uint32_t type, const lv_paged_cache &c, const
     d.tokens = b.tokens;
     d.group = group;
     d.tile = 16 * p.tiles;
+    d.tile_log2 = p.tiles == 2 ? 5 : 4;
     d.kv_heads = c.kv_heads;
     d.window = s.window;
     d.chunk = s.chunk;

@@ -98,7 +98,7 @@ constexpr uint32_t kPagedStep = 128;
 constexpr uint32_t kPagedRunMin = 2;
 
 struct PagedDeal {
-    uint32_t seqs, tokens, group, tile, kv_heads, window, chunk, positions;
+    uint32_t seqs, tokens, group, tile, tile_log2, kv_heads, window, chunk, positions;
     uint32_t target;     // workgroups to share the work; 0: nothing is cut
 };
 // steps that a tile of a sequence walks at most: its keys, or as many as a window or a chunk and the tile's tokens cover, and a border on either side
@@ -110,10 +110,8 @@ LV_HD uint32_t paged_steps(const PagedDeal &d, const PagedSeq &s)
     if (d.chunk && d.chunk < keys && d.chunk + tokens < keys) keys = d.chunk + tokens;
     return keys == 0 ? 1 : (keys + kPagedStep - 1) / kPagedStep + 1;
 }
-LV_HD uint32_t paged_tiles(const PagedDeal &d, const PagedSeq &s)
-{
-    return (uint32_t)(((uint64_t)s.rows * d.group + d.tile - 1) / d.tile);
-}
+// `tile` is a power of two; a call's rows, tokens times heads, are fewer than 2^31
+LV_HD uint32_t paged_tiles(const PagedDeal &d, const PagedSeq &s) { return (s.rows * d.group + d.tile - 1) >> d.tile_log2; }
 // all_steps is a sum of floats, off by less than 1e-4 of itself for 65535 sequences: what that adds to an item count is below the 1 of paged_items
 LV_HD uint32_t paged_run(const PagedDeal &d, float all_steps)
 {

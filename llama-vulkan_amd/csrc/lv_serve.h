@@ -70,11 +70,11 @@ __global__ __launch_bounds__(256) void rotate_kernel(RotateArgs a)
             auto get = [&](uint64_t i) {
                 if (a.type == LV_F32) return static_cast<const float *>(a.x)[i];
                 const uint16_t v = static_cast<const uint16_t *>(a.x)[i];
-                return a.type == LV_F16 ? half_bits_to_float(v) : pg_bf16(v);
+                return a.type == LV_F16 ? half_bits_to_float(v) : __uint_as_float((uint32_t)v << 16);
             };
             auto set = [&](uint64_t i, float v) {
                 if (a.type == LV_F32) static_cast<float *>(a.out)[i] = v;
-                else static_cast<uint16_t *>(a.out)[i] = (uint16_t)pg_bits(v, a.type);
+                else static_cast<uint16_t *>(a.out)[i] = (uint16_t)pg_bits(v, a.type == LV_F16);
             };
             if (u >= turned) {
                 if (a.out != a.x) set(to + at + a.rot + u - turned, get(from + at + a.rot + u - turned));

@@ -199,6 +199,7 @@ int main()
         } else if (what == "deal") {
             lv::PagedDeal d{};
             std::cin >> d.seqs >> d.group >> d.tile >> d.kv_heads >> d.window >> d.chunk >> d.positions >> d.target;
+            while (1u << d.tile_log2 < d.tile) d.tile_log2++;
             std::vector<uint32_t> lens(d.seqs), news(d.seqs);
             for (uint32_t b = 0; b < d.seqs; b++) std::cin >> lens[b] >> news[b], d.tokens += news[b];
             float all = 0;
