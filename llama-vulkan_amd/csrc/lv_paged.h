@@ -702,6 +702,287 @@ __global__ __launch_bounds__(256, paged_rows_waves(D, CT, NQ, QT)) void paged_ro
     }
 }
 
+// ---- tiles: chunks of a prompt -------------------------------------------------------------------------------------------------------
+// A workgroup takes 128 rows of one key head, 32 a wave, and walks their keys in tiles of 64 that all four waves share, double-buffered in LDS by direct
+// loads; two workgroups a CU, so that one's softmax fills the other's products.  v_mfma_f32_32x32x16: S^T = K Q^T leaves 32 scores of one row in a lane
+// (and 32 in lane ^ 32), and eight registers in a row are an operand of O^T = V^T P^T whose other one comes through ds_read_b64_tr_b16.
+// A wave reads 32 KB of LDS and issues 32 products of 32 clocks for a tile, its share of the LDS's rate and a SIMD's: bound by both, then by the softmax's vector work.
+// The running maximum is a reference that follows the true one when that is 2^8 above it, so that most tiles do not rescale.
+// Weights enter the second product as one fp16 (2^-11) or bf16 (2^-8) number: beside a 16-bit result's own rounding, over all the keys of a row.
+typedef float pg_f16v __attribute__((ext_vector_type(16)));
+
+template <bool BF> __device__ __forceinline__ pg_f16v pg_mfma32(typename PgFrag<BF>::type a, typename PgFrag<BF>::type b, pg_f16v c)
+{
+    if constexpr (BF) return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+    else return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+}
+
+typedef const __attribute__((address_space(1))) void pg_glb;
+typedef __attribute__((address_space(3))) void pg_lds;
+
+constexpr int kPagedTileRows = 128;
+constexpr float paged_tile_lift(bool bf) { return bf ? 0.f : 6.f; }      // weights up to 2^(6 + 8) in fp16
+
+template <int D, bool BF>
+__global__ __launch_bounds__(256, 2) void paged_tile_kernel(PagedAttnArgs a)
+{
+    constexpr int KS = D / 16, DT = D / 32, CH = D / 8, ROW = 2 * D, STAGE = 2 * 64 * ROW, SLOW = 8;
+    constexpr float kLift = paged_tile_lift(BF);
+    typedef typename PgFrag<BF>::type Frag;
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[2 * STAGE];      // stage: 64 rows of keys, 64 of values
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l32 = lane & 31, hh = lane >> 5;
+    const uint32_t head = blockIdx.x % a.c.kv_heads, item = blockIdx.x / a.c.kv_heads;
+    const PagedItem it = paged_locate<false>(a, item, lane);
+    if (!it.any) return;
+    const uint32_t group = a.deal.group, rows = it.s.rows * group, r0 = it.tile * kPagedTileRows, psize = 1u << a.c.shift;
+
+    // keys that rows first .. last see, any of them and all of them
+    struct Range {
+        uint32_t lo, hi, all_lo, all_hi;
+    };
+    auto range = [&](uint32_t first, uint32_t last) {
+        const int32_t p0 = it.s.pos0 + (int32_t)(first / group), p1 = it.s.pos0 + (int32_t)(last / group);
+        Range r;
+        r.lo = p0 >= 0 ? paged_first_key((uint32_t)p0, a.deal.window, a.deal.chunk) : 0;
+        r.hi = p1 >= 0 ? min((uint32_t)p1 + 1, it.s.keys) : 0;
+        r.all_lo = p1 >= 0 ? paged_first_key((uint32_t)p1, a.deal.window, a.deal.chunk) : 0;
+        r.all_hi = p0 >= 0 ? min((uint32_t)p0 + 1, it.s.keys) : 0;
+        return r;
+    };
+    const Range all = range(r0, min(r0 + kPagedTileRows, rows) - 1);
+    const uint32_t w0 = r0 + wave * 32;
+    const bool idle = w0 >= rows;      // no row of this wave: it brings its share of the tiles
+    const Range own = range(idle ? r0 : w0, min(w0 + 32, rows) - 1);
+    const uint32_t base = all.lo & ~31u, n_steps = all.hi > base ? (all.hi - base + kPagedStep - 1) / kPagedStep : 0;
+    const uint32_t s0 = min((uint64_t)it.part * it.run, (uint64_t)n_steps), s1 = min((uint64_t)s0 + it.run, (uint64_t)n_steps);
+    const uint32_t tiles = n_steps ? (all.hi - base + 63) / 64 : 0, t_end = min(s1 * (kPagedStep / 64), tiles);
+    const uint32_t *table = a.table + (uint64_t)it.seq * a.table_ld;
+
+    // a wave brings 16 keys and their values, which lie in one page.  Chunks of 16 bytes are stored at places that depend on their row: keys are read by 32 rows at
+    // once (chunk ^ row % 16), values by 4 rows x 64 bytes (groups of four chunks ^ row % 4; of two rows in 256 bytes, ^ half the row)
+    constexpr int PER = 64 / CH, LOADS = 16 / PER;      // rows a load, loads
+    auto issue = [&](int st, uint32_t page, uint32_t in) {
+        const uint8_t *keys = a.c.data + ((uint64_t)(page != kNoPage ? page : 0) * a.c.kv_heads + head) * a.c.block + in * ROW, *vals = keys + a.c.half;
+        uint8_t *kd = lds + st * STAGE + wave * (16 * ROW), *vd = kd + 64 * ROW;
+#pragma unroll
+        for (int i = 0; i < LOADS; i++) {
+            const int row = i * PER + lane / CH, ch = lane % CH;
+            const int kx = row % (CH < 16 ? CH : 16), vx = CH == 8 ? (row / 2 % 2) * 4 : (row % 4) * 4;
+            __builtin_amdgcn_global_load_lds((pg_glb *)(keys + (uint32_t)(row * ROW + (ch ^ kx) * 16)), (pg_lds *)(kd + i * 1024), 16, 0, 0);
+            __builtin_amdgcn_global_load_lds((pg_glb *)(vals + (uint32_t)(row * ROW + (ch ^ vx) * 16)), (pg_lds *)(vd + i * 1024), 16, 0, 0);
+        }
+    };
+    auto page_of = [&](uint32_t at) { return __builtin_amdgcn_readfirstlane(paged_page(a.c, table, a.table_ld, at)); };
+    uint32_t t = s0 * (kPagedStep / 64), mine = kNoPage;
+    if (t < t_end) issue(0, page_of(base + t * 64 + wave * 16), (base + t * 64 + wave * 16) & (psize - 1));
+    if (t + 1 < t_end) mine = page_of(base + (t + 1) * 64 + wave * 16);
+
+    // this lane's row
+    Frag q[KS];
+    float factor;
+    uint32_t lo, span;
+    {
+        const uint32_t r = w0 + l32;
+        const bool is = r < rows;
+        const uint32_t tk = is ? r / group : 0, h = head * group + (is ? r - tk * group : 0);
+        const int32_t p = it.s.pos0 + (int32_t)tk;
+        lo = p >= 0 ? paged_first_key((uint32_t)p, a.deal.window, a.deal.chunk) : 0;
+        const uint32_t end = p >= 0 ? min((uint32_t)p + 1, it.s.keys) : 0;
+        span = is && end > lo ? end - lo : 0;
+        float z[KS][8], top = 0.f;
+        pg_load_row<KS>(a.q, a.type, (uint64_t)(it.s.row0 + tk) * a.ldq + (uint64_t)h * D + hh * 8, 16, z);
+#pragma unroll
+        for (int k = 0; k < KS; k++)
+#pragma unroll
+            for (int e = 0; e < 8; e++) top = fmaxf(top, fabsf(z[k][e]));
+        top = fmaxf(top, __shfl_xor(top, 32, 64));
+        int e2 = (int)(__float_as_uint(top) >> 23) - 127 - 10;      // as in the kernel for rows
+        if (e2 > 117 || e2 < -110) e2 = 0;
+        const float down = copysignf(__uint_as_float((uint32_t)(127 - e2) << 23), a.scale);
+        factor = fmaxf(fabsf(a.scale) * __uint_as_float((uint32_t)(127 + e2) << 23), 1e-37f);      // above 0: -inf times it is -inf
+#pragma unroll
+        for (int k = 0; k < KS; k++)
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                Frag one[1];
+                pg_cut<BF, 1>(is ? z[k][e] * down : 0.f, e, one);
+                q[k][e] = one[0][e];
+            }
+    }
+
+    pg_f16v o[DT];
+#pragma unroll
+    for (int d = 0; d < DT; d++)
+#pragma unroll
+        for (int i = 0; i < 16; i++) o[d][i] = 0.f;
+    float m = -1e30f, l = 0.f;
+
+    int st = 0;
+    for (; t < t_end; t++, st ^= 1) {
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
+        if (t + 1 < t_end) {
+            issue(st ^ 1, mine, (base + (t + 1) * 64 + wave * 16) & (psize - 1));
+            if (t + 2 < t_end) mine = page_of(base + (t + 2) * 64 + wave * 16);
+        }
+        const uint32_t kb = base + t * 64;
+        uint32_t ok = 0;      // of 16 keys each: is there a page?
+#pragma unroll
+        for (int g = 0; g < 4; g++) ok |= (page_of(kb + 16 * g) != kNoPage ? 1u : 0u) << g;
+        uint8_t *kt_lds = lds + st * STAGE, *vt_lds = kt_lds + 64 * ROW;
+        int special = 0;
+        if (kb < all.all_lo || kb + 64 > all.all_hi || ok != 15) {
+            // some row does not see some key: values that no row sees become 0, and others are looked through for numbers that are not finite
+            uint32_t odd = 0;
+            for (int c = threadIdx.x; c < 64 * CH; c += 256) {
+                const uint32_t row = c / CH;
+                uint4 *w = reinterpret_cast<uint4 *>(vt_lds + c * 16);
+                if (kb + row - all.lo < ((ok >> (row / 16)) & 1 ? all.hi - all.lo : 0u)) odd |= pg_special<BF>(w->x) | pg_special<BF>(w->y) | pg_special<BF>(w->z) | pg_special<BF>(w->w);
+                else *w = make_uint4(0, 0, 0, 0);
+            }
+            special = __syncthreads_or(odd != 0);
+        }
+        if (idle || kb >= own.hi || kb + 64 <= own.lo) continue;
+        const bool edge = kb < own.all_lo || kb + 64 > own.all_hi || ok != 15;
+
+        pg_f16v sc[2];
+#pragma unroll
+        for (int kt = 0; kt < 2; kt++) {
+#pragma unroll
+            for (int i = 0; i < 16; i++) sc[kt][i] = 0.f;
+#pragma unroll
+            for (int k = 0; k < KS; k++) {
+                const int row = kt * 32 + l32;
+                const Frag f = *reinterpret_cast<const Frag *>(kt_lds + row * ROW + ((2 * k + hh) ^ (row % (CH < 16 ? CH : 16))) * 16);
+                sc[kt] = pg_mfma32<BF>(f, q[k], sc[kt]);
+            }
+        }
+        // score i of kt is key 32 kt + 8 (i / 4) + 4 hh + i % 4
+        const uint32_t first = kb + 4 * hh - lo;
+        if (edge) {
+#pragma unroll
+            for (int kt = 0; kt < 2; kt++)
+#pragma unroll
+                for (int i = 0; i < 16; i++) {
+                    const uint32_t sees = (ok >> (2 * kt + i / 8)) & 1 ? span : 0u;
+                    sc[kt][i] = first + (32 * kt + 8 * (i / 4) + i % 4) < sees ? sc[kt][i] : -INFINITY;
+                }
+        }
+        float top = -INFINITY;
+#pragma unroll
+        for (int kt = 0; kt < 2; kt++)
+#pragma unroll
+            for (int i = 0; i < 16; i += 2) top = fmaxf(fmaxf(sc[kt][i], sc[kt][i + 1]), top);
+        top = fmaxf(top, __shfl_xor(top, 32, 64)) * factor;
+        if (__any(top > m + SLOW)) {
+            const float to = fmaxf(top, m), f = pg_exp2(m - to);
+            m = to;
+            l *= f;
+#pragma unroll
+            for (int d = 0; d < DT; d++)
+#pragma unroll
+                for (int i = 0; i < 16; i++) o[d][i] *= f;
+        }
+        const float less = kLift - m;
+        Frag p[4];      // 16 keys each
+        float sum = 0.f;
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                const float w = pg_exp2(fmaf(sc[j / 2][j % 2 * 8 + e], factor, less));
+                sum += w;
+                if constexpr (BF) p[j][e] = (__bf16)w;
+                else p[j][e] = (_Float16)w;
+            }
+        l += sum;
+        // values of 16 keys as the first operand for 32 dimensions: lane has dimension l32, keys 4 hh .. + 3 and 8 + 4 hh .. + 3
+        const int vrow = 4 * hh + (lane & 15) / 4, vx = CH == 8 ? (vrow / 2 % 2) * 4 : (vrow % 4) * 4, vch = (l32 / 16) * 2 + (lane & 3) / 2, voff = (lane & 1) * 8;
+        auto values = [&](int d, int j) {
+            const uint8_t *at = vt_lds + (16 * j + vrow) * ROW + ((4 * d + vch) ^ vx) * 16 + voff;
+            const pg_s4 u = pg_read_columns(at), v = pg_read_columns(at + 8 * ROW);
+            return __builtin_bit_cast(Frag, pg_s8{u[0], u[1], u[2], u[3], v[0], v[1], v[2], v[3]});
+        };
+        if (special) {
+            // kinds 1 to 3, NaN, inf and -inf: their counts among the keys that a row sees
+            for (int kind = 1; kind <= 3; kind++) {
+                const float add = kind == 1 ? __builtin_nanf("") : kind == 2 ? INFINITY : -INFINITY;
+#pragma unroll
+                for (int d = 0; d < DT; d++) {
+                    pg_f16v n;
+#pragma unroll
+                    for (int i = 0; i < 16; i++) n[i] = 0.f;
+                    for (int j = 0; j < 4; j++) {
+                        Frag one;
+#pragma unroll
+                        for (int e = 0; e < 8; e++) {
+                            const float w = first + (16 * j + 8 * (e / 4) + e % 4) < ((ok >> j) & 1 ? span : 0u) ? 1.f : 0.f;
+                            if constexpr (BF) one[e] = (__bf16)w;
+                            else one[e] = (_Float16)w;
+                        }
+                        n = pg_mfma32<BF>(pg_only<BF>(values(d, j), kind), one, n);
+                    }
+#pragma unroll
+                    for (int i = 0; i < 16; i++) o[d][i] += n[i] > 0.f ? add : 0.f;
+                }
+            }
+        }
+#pragma unroll
+        for (int d = 0; d < DT; d++)
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                Frag v = values(d, j);
+                if (special) v = pg_only<BF>(v, 0);
+                o[d] = pg_mfma32<BF>(v, p[j], o[d]);
+            }
+    }
+
+    l += __shfl_xor(l, 32, 64);
+    const uint32_t r = w0 + l32;
+    if (r >= rows) return;
+    // register i of d is dimension 32 d + 8 (i / 4) + 4 hh + i % 4
+    if (it.parts > 1) {
+        const uint64_t at = ((uint64_t)item * a.c.kv_heads + head) * kPagedTileRows + wave * 32 + l32;
+#pragma unroll
+        for (int d = 0; d < DT; d++)
+#pragma unroll
+            for (int i = 0; i < 16; i += 4)
+                *reinterpret_cast<float4 *>(a.part + at * D + 32 * d + 2 * i + 4 * hh) = make_float4(o[d][i], o[d][i + 1], o[d][i + 2], o[d][i + 3]);
+        if (hh == 0) {
+            a.part_ml[2 * at] = m;
+            a.part_ml[2 * at + 1] = l;
+        }
+        return;
+    }
+    const uint32_t tk = r / group, h = head * group + (r - tk * group);
+    float f = 1.f;
+    if (a.sinks) {
+        const float sink = a.sinks[h] * 1.44269504088896341f, over = fmaxf(m, sink);
+        f = pg_exp2(m - over);
+        l = fmaf(l, f, pg_exp2(sink - over + kLift));
+    }
+    f = l == 0.f ? 0.f : f / l;
+    uint16_t *out = static_cast<uint16_t *>(a.out) + (uint64_t)(it.s.row0 + tk) * a.ldo + (uint64_t)h * D;
+    const bool half = a.type == LV_F16;
+#pragma unroll
+    for (int d = 0; d < DT; d++)
+#pragma unroll
+        for (int i = 0; i < 16; i += 4) {
+            float y[4];
+#pragma unroll
+            for (int e = 0; e < 4; e++) y[e] = l == 0.f ? 0.f : o[d][i + e] * f;
+            uint32_t lo2, hi2;
+            if (half) {
+                lo2 = pg_bits(y[0], true) | (pg_bits(y[1], true) << 16);
+                hi2 = pg_bits(y[2], true) | (pg_bits(y[3], true) << 16);
+            } else {
+                lo2 = pg_bits(y[0], false) | (pg_bits(y[1], false) << 16);
+                hi2 = pg_bits(y[2], false) | (pg_bits(y[3], false) << 16);
+            }
+            *reinterpret_cast<uint2 *>(out + 32 * d + 2 * i + 4 * hh) = make_uint2(lo2, hi2);
+        }
+}
+
 // ---- the parts of cut items put together: a workgroup a row ------------------------------------------------------------------------
 template <int D>
 __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttnArgs a, float lift)

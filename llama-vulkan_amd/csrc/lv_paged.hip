@@ -10,31 +10,34 @@ namespace {
 
 struct AttnPlan {
     PagedAttnArgs args{};
-    uint32_t tiles;                  // of 16 rows a workgroup
+    uint32_t tiles;                  // of 16 rows a workgroup; 8: the kernel for tiles
     uint32_t pieces;                 // of a query
     uint64_t items, part_floats, bytes;
 };
 
 // Workgroups that share the work of a call.  
 constexpr uint32_t kTargetPerUnit = 4;
+constexpr uint32_t kTileRowsMin = 48;
 
 AttnPlan attn_plan(uint32_t units, uint32_t type, const lv_paged_cache &c, const lv_paged_batch &b, const lv_paged_attn_spec &s)
 {
     AttnPlan p;
     PagedDeal &d = p.args.deal;
     const uint32_t group = s.heads / c.kv_heads;
-    p.tiles = c.dim <= 128 && (uint64_t)b.tokens * group > 16ull * b.seqs ? 2 : 1;
+    const uint64_t mean = (uint64_t)b.tokens * group / b.seqs;      // rows of a sequence and key head
     p.pieces = type == LV_F32 ? (c.type == LV_BF16 ? 3 : 2) : type == LV_F16 && c.type == LV_BF16 ? 3 : 1;
+    const bool tile = p.pieces == 1 && (c.type == LV_F16 || c.type == LV_BF16) && (c.dim == 64 || c.dim == 128) && mean >= kTileRowsMin;
+    p.tiles = tile ? 8 : c.dim <= 128 && mean > 16 ? 2 : 1;
     d.seqs = b.seqs;
     d.tokens = b.tokens;
     d.group = group;
     d.tile = 16 * p.tiles;
-    d.tile_log2 = p.tiles == 2 ? 5 : 4;
+    d.tile_log2 = tile ? 7 : p.tiles == 2 ? 5 : 4;
     d.kv_heads = c.kv_heads;
     d.window = s.window;
     d.chunk = s.chunk;
     d.positions = b.table_ld * c.page;
-    d.target = kTargetPerUnit * units;
+    d.target = (tile ? 2 : kTargetPerUnit) * units;
     if ((uint64_t)b.tokens * group / d.tile * c.kv_heads >= d.target) d.target = 0;
     p.items = paged_items(d);
     p.part_floats = d.target ? p.items * c.kv_heads * d.tile * c.dim : 0;
@@ -58,13 +61,21 @@ template <int D>
 void launch_attention(const AttnPlan &p, uint32_t grid, hipStream_t st)
 {
     const PagedAttnArgs &a = p.args;
-    switch (a.c.type) {
+    const bool bf = a.c.type == LV_BF16;
+    float lift = bf ? 0.f : 12.f;
+    if (p.tiles == 8) {
+        lift = paged_tile_lift(bf);
+        if constexpr (D == 64 || D == 128) {
+            if (bf) paged_tile_kernel<D, true><<<dim3(grid), dim3(256), 0, st>>>(a);
+            else paged_tile_kernel<D, false><<<dim3(grid), dim3(256), 0, st>>>(a);
+        }
+    } else switch (a.c.type) {
     case LV_F16: p.pieces == 1 ? launch_rows<D, kPgF16, 1>(p, grid, st) : launch_rows<D, kPgF16, 2>(p, grid, st); break;
     case LV_BF16: p.pieces == 1 ? launch_rows<D, kPgBf16, 1>(p, grid, st) : launch_rows<D, kPgBf16, 3>(p, grid, st); break;
     case LV_Q8_0: p.pieces == 1 ? launch_rows<D, kPgQ8, 1>(p, grid, st) : launch_rows<D, kPgQ8, 2>(p, grid, st); break;
     default: p.pieces == 1 ? launch_rows<D, kPgQ4, 1>(p, grid, st) : launch_rows<D, kPgQ4, 2>(p, grid, st); break;
     }
-    if (a.deal.target) paged_join_kernel<D><<<dim3(a.deal.tokens * a.deal.group * a.deal.kv_heads), dim3(256), 0, st>>>(a, a.c.type == LV_BF16 ? 0.f : 12.f);
+    if (a.deal.target) paged_join_kernel<D><<<dim3(a.deal.tokens * a.deal.group * a.deal.kv_heads), dim3(256), 0, st>>>(a, lift);
 }
 
 }  // namespace

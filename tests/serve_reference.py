@@ -187,20 +187,21 @@ def attention(pool, step, q, heads, scale, window=0, chunk=0, sinks=None):
 def attention_bound(want, size, reach, seen, mass, dim, kind, cache):
     """How far a kernel's result may be off.  Scores: products of exact operands (32-bit queries as pieces of 22 bits or more) summed in fp32, dim + 8 roundings of at most
     2^-24 of sum |q k|, 2^-22 for the pieces; an error e of a score is one of e (and e of the maximum) in a weight's exponent.  Weights: exp2 to 2^-22, the sum over `seen` keys in
-    fp32, and rounded to the matrix cores' operands: fp16 2^-11, two pieces of bf16 2^-16, two of fp16 2^-22.  Values of blocks are scaled in fp16 (2^-11) where the result is
+    fp32, and rounded to the matrix cores' operands: fp16 2^-11, bf16 2^-8 where the result is bf16 too (two pieces of it 2^-16), two pieces of fp16 2^-22.  Values of blocks are scaled in fp16 (2^-11) where the result is
     16-bit.  The sums over keys are fp32 (`seen` roundings at most), then the result is rounded once.
-    Numbers next to 0: weights enter fp16 products in units where a row's largest one (of some 32 keys' turn) is 2^12, and below 2^-14 a rounding is one of 2^-25 whatever the
-    number, so each weight may be off by 2^-37 of the largest, which is no more than the sum: 2^-37 sum |v| of the result.  Scaled 16-bit values: 2^-25 times weights of sum 1."""
+    Numbers next to 0: weights enter fp16 products in units where a row's largest one (of the keys so far) is 2^12, in the kernel for chunks, whose results are 16-bit, 2^6 to 2^14.
+    Below 2^-14 a rounding is one of 2^-25 whatever the number, so each weight may be off by 2^-37 or 2^-31 of the largest, which is no more than the sum: so much times sum |v| of the
+    result.  Scaled 16-bit values: 2^-25 times weights of sum 1."""
     blocks = cache in (Q8, Q4)
     if kind == F32:
         weight, value = 2.0 ** -21, 0.0
     elif cache == BF16:
-        weight, value = 2.0 ** -16, 0.0
+        weight, value = 2.0 ** -8 if kind == BF16 else 2.0 ** -16, 0.0
     else:
         weight, value = 2.0 ** -11, 2.0 ** -11 if blocks else 0.0
     score = reach[..., None] * ((dim + 8) * 2.0 ** -24 + 2.0 ** -22)
     relative = 2 * score + 2.0 ** -20 + 2 * (seen[:, None, None] + 64) * 2.0 ** -24 + weight + value
-    small = (0 if cache == BF16 else 2.0 ** -37 * mass) + (2.0 ** -25 if value else 0)
+    small = (0 if cache == BF16 else (2.0 ** -37 if kind == F32 else 2.0 ** -31) * mass) + (2.0 ** -25 if value else 0)
     return HALF_STEP[kind] * np.abs(want) * 1.01 + relative * (1 + relative) * 1.1 * size + small + (2.0 ** -24 if kind == F16 else 1e-37)
 
 

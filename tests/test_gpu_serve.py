@@ -330,6 +330,58 @@ def test_attention_of_numbers_that_are_not_finite(dev, kind, cache):
     assert np.isfinite(want[:30]).all() and np.isinf(want[30]).any() and np.isnan(want[36:40]).any()
 
 
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("cache,kind", [(F16, F16), (F16, BF16), (BF16, BF16)], ids=lambda k: ref.NAMES[k])
+def test_attention_of_numbers_that_are_not_finite_in_chunks(dev, cache, kind, dim):
+    def edit(pool, step):
+        for b, p, which, at, x in [(0, 30, 1, 3, np.inf), (0, 70, 1, 3, np.nan), (0, 71, 1, 40, -np.inf), (0, 75, 0, 0, np.nan), (1, 209, 1, 7, np.inf), (1, 5, 1, 8, -np.inf),
+                                   (1, 190, 1, 63, np.nan)]:
+            page, i = step.place(pool, b, p)
+            codes, _ = pool.row(page, 0, which, i)
+            codes.view(np.uint16)[at] = ref.encode(np.float32([x]), pool.kind).view(np.uint16)[0]
+    got, want = check_attention(dev, np.random.default_rng(45), cache, kind, 2, 1, dim, 16, [80, 210], [80, 45], edit=edit)
+    assert np.isfinite(want[:30]).all() and np.isinf(want[30]).any() and np.isnan(want[75:80]).any()
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("cache,kind,window", [(F16, F16, 0), (BF16, BF16, 0), (F16, BF16, 700), (Q8, F16, 0)], ids=str)
+def test_attention_of_a_chunk_behind_a_long_context(dev, cache, kind, window, dim):
+    """few tiles of many keys: cut into parts"""
+    check_attention(dev, np.random.default_rng(46), cache, kind, 4, 1, dim, 128, [1900, 333], [41, 10], window=window, sinks=True, pad=2)
+
+
+def test_attention_of_chunks_without_pages(dev):
+    def edit(pool, step):
+        step.table[0, 2] = pool.pages
+        step.table[0, 5] = NO_PAGE
+        step.table[1, :] = 0xFFFFFF00
+        step.lens[2] = 30                   # fewer than the new ones
+    for sinks in (False, True):
+        got, want = check_attention(dev, np.random.default_rng(47), F16, F16, 2, 2, 64, 16, [130, 50, 70], [90, 40, 70], sinks=sinks, edit=edit)
+        assert not got[90:130].any() and not got[130:170].any() and got[170:].any() and got[:90].any()
+
+
+@pytest.mark.parametrize("cache", [F16, BF16], **KINDS)
+def test_attention_of_chunks_of_large_scores(dev, cache):
+    """the reference of a row's weights is moved often, and by a lot"""
+    check_attention(dev, np.random.default_rng(48), cache, BF16 if cache == BF16 else F16, 2, 1, 128, 16, [300, 177], [200, 177], spread=40)
+
+
+@pytest.mark.parametrize("scale", [-0.2, 0.0])
+@pytest.mark.parametrize("new", [1, 60])
+def test_attention_scales(dev, scale, new):
+    rng = np.random.default_rng(49)
+    pool = ref.Pool(F16, 1, 64, 16, 12, rng)
+    step = ref.Step(pool, [150], [new], rng)
+    for p in range(150):
+        at = step.place(pool, 0, p)
+        for which in (0, 1):
+            pool.put(at[0], 0, which, at[1], rng.standard_normal(64))
+    got, held = run_attention(dev, pool, step, rng.standard_normal((new, 2, 64)), F16, 2, scale)
+    want, size, reach, seen, mass = ref.attention(pool, step, held, 2, float(np.float32(scale)))
+    assert np.all(np.abs(got - want) <= ref.attention_bound(want, size, reach, seen, mass, 64, F16, F16))
+
+
 @pytest.mark.parametrize("cache", [F16, Q8], **KINDS)
 def test_attention_without_pages(dev, cache):
     """keys whose page is not in the pool are hidden; a row that sees nothing is 0, also beside a sink"""
