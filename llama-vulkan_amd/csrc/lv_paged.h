@@ -37,6 +37,16 @@ struct PagedAttnArgs {
     float *part, *part_ml;      // of cut items: [item][kv head][tile][dim], [item][kv head][tile][2]
 };
 
+// paged_page of a position that is the same in all lanes: as constant memory the table is read by scalar loads, which wait for nothing but themselves.  A vector
+// load's wait is one for all loads before it: keys and values on their way.
+__device__ __forceinline__ uint32_t paged_page_uniform(const PagedAttnArgs &a, const uint32_t *row, uint32_t position)
+{
+    const uint32_t at = __builtin_amdgcn_readfirstlane(position), i = at >> a.c.shift;
+    uint32_t p = kNoPage;
+    if (i < a.table_ld) p = *((const __attribute__((address_space(4))) uint32_t *)(uintptr_t)(row + i));
+    return p < a.c.pages ? p : kNoPage;
+}
+
 // ---- which item ------------------------------------------------------------------------------------------------------------------
 struct PagedItem {
     PagedSeq s;
@@ -364,7 +374,7 @@ __global__ __launch_bounds__(256, paged_rows_waves(D, CT, NQ, QT)) void paged_ro
     // where 16 keys' codes lie (of keys; of values and scales at the same distances in every block), null without a page
     Turn x;
     auto place = [&](uint32_t t, int kt, uint32_t &in) {
-        const uint32_t at = base + t * 32 + 16 * kt, page = __builtin_amdgcn_readfirstlane(paged_page(a.c, table, a.table_ld, at));
+        const uint32_t at = base + t * 32 + 16 * kt, page = paged_page_uniform(a, table, at);
         in = at & (psize - 1);
         return page;
     };
@@ -772,7 +782,7 @@ __global__ __launch_bounds__(256, 2) void paged_tile_kernel(PagedAttnArgs a)
             __builtin_amdgcn_global_load_lds((pg_glb *)(vals + (uint32_t)(row * ROW + (ch ^ vx) * 16)), (pg_lds *)(vd + i * 1024), 16, 0, 0);
         }
     };
-    auto page_of = [&](uint32_t at) { return __builtin_amdgcn_readfirstlane(paged_page(a.c, table, a.table_ld, at)); };
+    auto page_of = [&](uint32_t at) { return paged_page_uniform(a, table, at); };
     uint32_t t = s0 * (kPagedStep / 64), mine = kNoPage;
     if (t < t_end) issue(0, page_of(base + t * 64 + wave * 16), (base + t * 64 + wave * 16) & (psize - 1));
     if (t + 1 < t_end) mine = page_of(base + (t + 1) * 64 + wave * 16);

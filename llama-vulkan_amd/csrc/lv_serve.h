@@ -98,117 +98,179 @@ struct PagedRowsArgs {
     uint32_t ldk, ldv, type;
 };
 
-// where a row's token lies: the page, or kNoPage, and the place in it.  By every wave on its own; `row` is the same in all lanes
-__device__ __forceinline__ uint32_t paged_place(const PagedRowsArgs &a, uint32_t row, uint32_t &in)
+// where the tokens of rows row0 + lane lie: the page, or kNoPage, and the place in it.  By a whole wave; lanes from `rows` on find nothing
+__device__ __forceinline__ uint2 paged_places(const PagedRowsArgs &a, uint32_t row0, uint32_t rows, uint32_t lane)
 {
-    const int lane = threadIdx.x & 63;
+    // the last sequence that starts at row0 or before it: 64 at a time; then, where a lane's row is not that sequence's, by halves
+    uint32_t first = 0;
     for (uint32_t b0 = 0; b0 < a.seqs; b0 += 64) {
-        PagedSeq s{};
-        uint32_t page = kNoPage, at = 0;
-        if (b0 + lane < a.seqs) s = paged_seq(a.starts[b0 + lane], a.starts[b0 + lane + 1], a.lens[b0 + lane], a.tokens, a.positions);
-        const bool mine = row >= s.row0 && row - s.row0 < s.rows;
-        if (mine) {
-            const int32_t p = s.pos0 + (int32_t)(row - s.row0);
-            if (p >= 0) {
-                page = paged_page(a.c, a.table + (uint64_t)(b0 + lane) * a.table_ld, a.table_ld, (uint32_t)p);
-                at = (uint32_t)p & ((1u << a.c.shift) - 1);
-            }
-        }
-        const uint64_t here = __ballot(mine);
-        if (here) {
-            const int l = __builtin_ctzll(here);
-            in = __builtin_amdgcn_readlane(at, l);
-            return __builtin_amdgcn_readlane(page, l);
-        }
+        const uint64_t from_here = __ballot(b0 + lane < a.seqs && a.starts[min(b0 + lane, a.seqs)] <= row0);
+        if (from_here) first = b0 + 63 - __builtin_clzll(from_here);
+        if (from_here != ~0ull) break;
     }
-    return kNoPage;
+    uint2 out = make_uint2(kNoPage, 0);
+    if (lane >= rows) return out;
+    const uint32_t row = row0 + lane;
+    uint32_t b = first, n = a.starts[first + 1] <= row ? a.seqs - first : 1;
+    while (n > 1) {
+        const uint32_t half = n / 2;
+        const bool up = a.starts[b + half] <= row;
+        b = up ? b + half : b;
+        n = up ? n - half : half;
+    }
+    const PagedSeq s = paged_seq(a.starts[b], a.starts[b + 1], a.lens[b], a.tokens, a.positions);
+    if (row < s.row0 || row - s.row0 >= s.rows) return out;
+    const int32_t p = s.pos0 + (int32_t)(row - s.row0);
+    if (p < 0) return out;
+    out.x = paged_page(a.c, a.table + (uint64_t)b * a.table_ld, a.table_ld, (uint32_t)p);
+    out.y = (uint32_t)p & ((1u << a.c.shift) - 1);
+    return out;
 }
 
-// A thread takes eight elements, four neighbouring threads a block of 32.  grid (tokens, units / 256).  Bound by the bytes of the rows.
-template <bool WRITE>
-__global__ __launch_bounds__(256) void paged_copy_kernel(PagedRowsArgs a)
+// eight numbers of a block of 32 as it is stored; the block's are in four neighbouring threads, `quarter` says which
+__device__ __forceinline__ void paged_put_block(const float (&x)[8], bool eight, uint32_t quarter, uint8_t *block_codes, uint16_t *scale)
 {
-    const uint32_t per = a.c.dim / 8, units = 2 * a.c.kv_heads * per, u = blockIdx.y * 256 + threadIdx.x, row = blockIdx.x;
-    const bool mine = u < units;
-    const uint32_t which = u >= units / 2 ? 1 : 0, w = u - which * (units / 2), head = w / per, d = (w - head * per) * 8;
-    const uint64_t at = (uint64_t)row * (which ? a.ldv : a.ldk) + (uint64_t)w * 8;
-    void *rows = which ? a.v : a.k;
-    float x[8];
-    if (WRITE && mine) pg_load8(rows, a.type, at, x);      // on its way while the page is looked up
-    uint32_t in = 0;
-    const uint32_t page = paged_place(a, row, in);
-    if (page == kNoPage || !mine) return;      // whole groups of four: units is a multiple of 8
-    uint8_t *codes = a.c.data + paged_codes(a.c, page, head, which, in), *scales = a.c.data + paged_scales(a.c, page, head, which, in);
-    if (a.c.type == LV_F16 || a.c.type == LV_BF16) {
-        if constexpr (WRITE) {
-            pg_store8(codes, a.c.type, d, x);
-        } else {
-            pg_load8(codes, a.c.type, d, x);
-            pg_store8(rows, a.type, at, x);
-        }
+    float hi = -INFINITY, lo = INFINITY;
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+        hi = fmaxf(hi, x[e]);      // of a number and NaN, the number
+        lo = fminf(lo, x[e]);
+    }
+    hi = fmaxf(hi, dpp_mov<0xB1>(hi));
+    hi = fmaxf(hi, dpp_mov<0x4E>(hi));
+    lo = fminf(lo, dpp_mov<0xB1>(lo));
+    lo = fminf(lo, dpp_mov<0x4E>(lo));
+    if (hi < lo) hi = lo = 0.f;      // nothing but NaN
+    float s;
+    if (eight) s = fminf(fmaxf(hi, -lo) * (1.f / 127.f), 515.5f);
+    else s = fminf(fmaxf((hi >= -lo ? hi : lo) * -0.125f, -8188.f), 8188.f);
+    uint16_t h = float_to_half_bits(s);
+    if ((h & 0x7fffu) == 0) h = 0;
+    const float back = half_bits_to_float(h), inv = back == 0.f ? 0.f : 1.f / back;
+    const float low = eight ? -127.f : -8.f, high = eight ? 127.f : 7.f;
+    uint32_t lo4 = 0, hi4 = 0;
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+        const float c = inv == 0.f ? 0.f : fminf(fmaxf(rintf(x[e] * inv), low), high);      // inf times 0 is no number
+        const int q = x[e] == x[e] ? (int)c : 0;
+        const uint32_t bits = (eight ? (uint32_t)q & 0xffu : (uint32_t)(q + 8) & 0xfu) << (8 * (e % 4));
+        if (e < 4) lo4 |= bits;
+        else hi4 |= bits;
+    }
+    if (quarter == 0) *scale = h;
+    if (eight) {
+        *reinterpret_cast<uint2 *>(block_codes + quarter * 8) = make_uint2(lo4, hi4);
         return;
     }
-    const bool eight = a.c.type == LV_Q8_0;
-    uint16_t *scale = reinterpret_cast<uint16_t *>(scales) + d / 32;
-    const uint32_t quarter = d / 8 % 4;      // of the block
+    // the first two of four hold elements 0 .. 15 and get 16 .. 31 from the other two
+    const uint32_t up_lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)lo4, 0xEE, 0xf, 0xf, true);
+    const uint32_t up_hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)hi4, 0xEE, 0xf, 0xf, true);
+    if (quarter < 2) *reinterpret_cast<uint2 *>(block_codes + quarter * 8) = make_uint2(lo4 | (up_lo << 4), hi4 | (up_hi << 4));
+}
+
+// A unit is eight elements of a token's keys or values, four neighbouring threads have a block of 32.  A workgroup takes `run` tokens, up to 1024 units of them, and
+// asks for four units a thread before it uses the first: with one token a workgroup the look-up of its page, three loads in a row, was most of a copy's time
+// (16001-token sequences of 8 bits read back: 85 us).  grid (tokens / run, units of a token / 1024).  Bound by the bytes of the rows.
+constexpr uint32_t kCopyUnits = 4, kCopyRun = 64;
+
+// Workgroup i of n as a place in 0 .. n - 1 such that the workgroups of one XCD, every eighth, get neighbouring places: a token's scales, and its codes of 4 bits,
+// fill less than a line of the cache, and lines that two XCDs write go to memory twice.
+__device__ __forceinline__ uint32_t paged_eighth(uint32_t i, uint32_t n)
+{
+    const uint32_t x = i % 8, q = n / 8, r = n % 8;
+    return x * q + min(x, r) + i / 8;
+}
+
+template <bool WRITE>
+__global__ __launch_bounds__(256) void paged_copy_kernel(PagedRowsArgs a, uint32_t run)
+{
+    __shared__ uint2 places[kCopyRun];
+    const uint32_t per = a.c.dim / 8, half = a.c.kv_heads * per, units = 2 * half, row0 = paged_eighth(blockIdx.x, gridDim.x) * run, u0 = blockIdx.y * 256 * kCopyUnits;
+    const uint32_t rows = min(run, a.tokens - row0), width = min(units - u0, 256 * kCopyUnits), all = rows * width;      // run is 1 where a token has more units
+    const bool blocks = a.c.type == LV_Q8_0 || a.c.type == LV_Q4_0, eight = a.c.type == LV_Q8_0;
+    float x[kCopyUnits][8];
+    uint32_t row[kCopyUnits], u[kCopyUnits];
+    void *rows_at[kCopyUnits];
+    uint64_t at[kCopyUnits];
+#pragma unroll
+    for (uint32_t i = 0; i < kCopyUnits; i++) {
+        const uint32_t n = min(i * 256 + threadIdx.x, all - 1);
+        row[i] = n / width;
+        u[i] = u0 + n - row[i] * width;
+        const uint32_t which = u[i] >= half ? 1 : 0;
+        rows_at[i] = which ? a.v : a.k;
+        at[i] = (uint64_t)(row0 + row[i]) * (which ? a.ldv : a.ldk) + (uint64_t)(u[i] - which * half) * 8;
+    }
     if constexpr (WRITE) {
-        float hi = -INFINITY, lo = INFINITY;
+        if (a.type == LV_F32) {
 #pragma unroll
-        for (int e = 0; e < 8; e++) {
-            hi = fmaxf(hi, x[e]);      // of a number and NaN, the number
-            lo = fminf(lo, x[e]);
-        }
-        hi = fmaxf(hi, dpp_mov<0xB1>(hi));
-        hi = fmaxf(hi, dpp_mov<0x4E>(hi));
-        lo = fminf(lo, dpp_mov<0xB1>(lo));
-        lo = fminf(lo, dpp_mov<0x4E>(lo));
-        if (hi < lo) hi = lo = 0.f;      // nothing but NaN
-        float s;
-        if (eight) s = fminf(fmaxf(hi, -lo) * (1.f / 127.f), 515.5f);
-        else s = fminf(fmaxf((hi >= -lo ? hi : lo) * -0.125f, -8188.f), 8188.f);
-        uint16_t h = float_to_half_bits(s);
-        if ((h & 0x7fffu) == 0) h = 0;
-        const float back = half_bits_to_float(h), inv = back == 0.f ? 0.f : 1.f / back;
-        int q[8];
-#pragma unroll
-        for (int e = 0; e < 8; e++) {
-            const float c = rintf(x[e] * inv);
-            q[e] = x[e] == x[e] && inv != 0.f ? (int)fminf(fmaxf(c, eight ? -127.f : -8.f), eight ? 127.f : 7.f) : 0;
-        }
-        if (quarter == 0) *scale = h;
-        if (eight) {
-            uint32_t lo4 = 0, hi4 = 0;
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-                lo4 |= ((uint32_t)q[e] & 0xffu) << (8 * e);
-                hi4 |= ((uint32_t)q[4 + e] & 0xffu) << (8 * e);
-            }
-            *reinterpret_cast<uint2 *>(codes + d) = make_uint2(lo4, hi4);
+            for (uint32_t i = 0; i < kCopyUnits; i++) pg_load8(rows_at[i], LV_F32, at[i], x[i]);
         } else {
-            uint32_t lo4 = 0, hi4 = 0;
+            uint4 w[kCopyUnits];
 #pragma unroll
-            for (int e = 0; e < 4; e++) {
-                lo4 |= ((uint32_t)(q[e] + 8) & 0xfu) << (8 * e);
-                hi4 |= ((uint32_t)(q[4 + e] + 8) & 0xfu) << (8 * e);
+            for (uint32_t i = 0; i < kCopyUnits; i++) w[i] = *reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(rows_at[i]) + at[i]);
+#pragma unroll
+            for (uint32_t i = 0; i < kCopyUnits; i++) {
+                if (a.type == LV_F16) pg_unpack8<false>(w[i], x[i]);
+                else pg_unpack8<true>(w[i], x[i]);
             }
-            // lanes 0 and 1 of four hold elements 0 .. 15 and get 16 .. 31 from lanes 2 and 3
-            const uint32_t up_lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)lo4, 0xEE, 0xf, 0xf, true);
-            const uint32_t up_hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)hi4, 0xEE, 0xf, 0xf, true);
-            if (quarter < 2) *reinterpret_cast<uint2 *>(codes + d / 32 * 16 + quarter * 8) = make_uint2(lo4 | (up_lo << 4), hi4 | (up_hi << 4));
+        }
+    }
+    if (threadIdx.x < 64) {
+        const uint2 p = paged_places(a, row0, rows, threadIdx.x);
+        if (threadIdx.x < rows) places[threadIdx.x] = p;
+    }
+    __syncthreads();
+    uint8_t *codes[kCopyUnits], *scales[kCopyUnits];
+    bool mine[kCopyUnits];
+    uint32_t d[kCopyUnits];
+#pragma unroll
+    for (uint32_t i = 0; i < kCopyUnits; i++) {
+        const uint2 p = places[row[i]];
+        const uint32_t which = u[i] >= half ? 1 : 0, w = u[i] - which * half, head = w / per;
+        d[i] = (w - head * per) * 8;
+        mine[i] = i * 256 + threadIdx.x < all && p.x != kNoPage;      // whole groups of four: units and width are multiples of 8
+        const uint32_t page = p.x != kNoPage ? p.x : 0;
+        codes[i] = a.c.data + paged_codes(a.c, page, head, which, p.y);
+        scales[i] = a.c.data + paged_scales(a.c, page, head, which, p.y) + d[i] / 32 * 2;
+    }
+    if constexpr (WRITE) {
+#pragma unroll
+        for (uint32_t i = 0; i < kCopyUnits; i++) {
+            if (!mine[i]) continue;
+            if (blocks) paged_put_block(x[i], eight, d[i] / 8 % 4, codes[i] + d[i] / 32 * (eight ? 32 : 16), reinterpret_cast<uint16_t *>(scales[i]));
+            else pg_store8(codes[i], a.c.type, d[i], x[i]);
         }
     } else {
-        const float s = half_bits_to_float(*scale);
-        if (eight) {
-            const uint2 q = *reinterpret_cast<const uint2 *>(codes + d);
+        uint4 w[kCopyUnits];
+        uint16_t s[kCopyUnits];
+        if (!blocks) {
 #pragma unroll
-            for (int e = 0; e < 8; e++) x[e] = s * (float)(int8_t)((e < 4 ? q.x : q.y) >> (8 * (e % 4)));
+            for (uint32_t i = 0; i < kCopyUnits; i++) w[i] = *reinterpret_cast<const uint4 *>(codes[i] + d[i] * 2);
         } else {
-            const uint2 q = *reinterpret_cast<const uint2 *>(codes + d / 32 * 16 + quarter % 2 * 8);
-            const int shift = quarter < 2 ? 0 : 4;
 #pragma unroll
-            for (int e = 0; e < 8; e++) x[e] = s * (float)((int)(((e < 4 ? q.x : q.y) >> (8 * (e % 4) + shift)) & 0xfu) - 8);
+            for (uint32_t i = 0; i < kCopyUnits; i++) {
+                const uint2 q = *reinterpret_cast<const uint2 *>(codes[i] + (eight ? d[i] : d[i] / 32 * 16 + d[i] / 8 % 2 * 8));
+                w[i] = make_uint4(q.x, q.y, 0, 0);
+                s[i] = *reinterpret_cast<const uint16_t *>(scales[i]);
+            }
         }
-        pg_store8(rows, a.type, at, x);
+#pragma unroll
+        for (uint32_t i = 0; i < kCopyUnits; i++) {
+            if (!blocks) {
+                if (a.c.type == LV_F16) pg_unpack8<false>(w[i], x[i]);
+                else pg_unpack8<true>(w[i], x[i]);
+            } else {
+                const float f = half_bits_to_float(s[i]);
+                const int shift = d[i] / 8 % 4 < 2 ? 0 : 4;
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    const uint32_t b = (e < 4 ? w[i].x : w[i].y) >> (8 * (e % 4));
+                    x[i][e] = f * (float)(eight ? (int)(int8_t)b : (int)((b >> shift) & 0xfu) - 8);
+                }
+            }
+            if (mine[i]) pg_store8(rows_at[i], a.type, at[i], x[i]);
+        }
     }
 }
 
@@ -242,8 +304,9 @@ __device__ __forceinline__ uint32_t verify_standing(const lv_draft_batch &b, uin
 }
 
 struct VerifyRow {
-    const float *p, *q;        // q null: nothing, or with `x` below vocab the draft was picked and only its own token is taken out
+    const float *p, *q;        // q null: nothing is taken off but, with `x` below vocab, the one token that was picked
     uint32_t x;
+    bool wide;                 // rows of 16-byte alignment
 };
 __device__ __forceinline__ VerifyRow verify_row(const lv_draft_batch &b, uint32_t seq, uint32_t r, uint32_t count)
 {
@@ -251,14 +314,29 @@ __device__ __forceinline__ VerifyRow verify_row(const lv_draft_batch &b, uint32_
     v.p = b.target + ((uint64_t)seq * (b.drafts + 1) + r) * b.ld_target;
     v.q = r < count && b.draft ? b.draft + ((uint64_t)seq * b.drafts + r) * b.ld_draft : nullptr;
     v.x = r < count && !b.draft ? b.tokens[(uint64_t)seq * b.drafts + r] : 0xffffffffu;
+    v.wide = ((uintptr_t)v.p | (uintptr_t)v.q) % 16 == 0;
     return v;
 }
 __device__ __forceinline__ double verify_whole(float p) { return p > 0.f ? (double)p : 0.0; }
-__device__ __forceinline__ double verify_rest(const VerifyRow &v, uint32_t j, float p, float q)
+__device__ __forceinline__ double verify_rest(uint32_t picked, uint32_t j, float p, float q)
 {
-    if (j == v.x) return 0.0;
-    const double d = (double)p - (v.q ? (double)q : 0.0);
+    const double d = j == picked ? 0.0 : (double)p - (double)q;
     return d > 0.0 ? d : 0.0;
+}
+// entries j .. j + 3 of a row, j a multiple of 4; 0 from `end` on
+__device__ __forceinline__ void verify_load4(const VerifyRow &v, uint32_t j, uint32_t end, float (&p)[4], float (&q)[4])
+{
+    if (v.wide && j + 4 <= end) {
+        const float4 x = *reinterpret_cast<const float4 *>(v.p + j), y = v.q ? *reinterpret_cast<const float4 *>(v.q + j) : make_float4(0.f, 0.f, 0.f, 0.f);
+        p[0] = x.x; p[1] = x.y; p[2] = x.z; p[3] = x.w;
+        q[0] = y.x; q[1] = y.y; q[2] = y.z; q[3] = y.w;
+        return;
+    }
+#pragma unroll
+    for (uint32_t e = 0; e < 4; e++) {
+        p[e] = j + e < end ? v.p[j + e] : 0.f;
+        q[e] = v.q && j + e < end ? v.q[j + e] : 0.f;
+    }
 }
 
 __device__ __forceinline__ double wave_sum_double(double v)
@@ -276,11 +354,17 @@ __global__ __launch_bounds__(256) void verify_sums_kernel(VerifyArgs a)
     uint32_t count;
     const uint32_t r = verify_standing(a.b, seq, count);
     const VerifyRow row = verify_row(a.b, seq, r, count);
+    if (blockIdx.x == 0 && threadIdx.x == 0) a.accepted[seq] = r;
     double rest = 0.0, whole = 0.0;
-    for (uint32_t j = j0 + threadIdx.x; j < j1; j += 256) {
-        const float p = row.p[j], q = row.q ? row.q[j] : 0.f;
-        rest += verify_rest(row, j, p, q);
-        whole += verify_whole(p);
+#pragma unroll 2
+    for (uint32_t j = j0 + 4 * threadIdx.x; j < j1; j += 1024) {
+        float p[4], q[4];
+        verify_load4(row, j, j1, p, q);
+#pragma unroll
+        for (uint32_t e = 0; e < 4; e++) {
+            rest += verify_rest(row.x, j + e, p[e], q[e]);
+            whole += verify_whole(p[e]);
+        }
     }
     rest = wave_sum_double(rest);
     whole = wave_sum_double(whole);
@@ -292,14 +376,13 @@ __global__ __launch_bounds__(256) void verify_sums_kernel(VerifyArgs a)
     if (threadIdx.x < 2) a.sums[((uint64_t)seq * a.segments + blockIdx.x) * 2 + threadIdx.x] = (part[0][threadIdx.x] + part[1][threadIdx.x]) + (part[2][threadIdx.x] + part[3][threadIdx.x]);
 }
 
-// grid (seqs)
+// grid (seqs).  `accepted` is what the sums' launch found
 __global__ __launch_bounds__(256) void verify_pick_kernel(VerifyArgs a)
 {
     __shared__ double waves[4];
     __shared__ uint32_t found, last;
     const uint32_t seq = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    uint32_t count;
-    const uint32_t r = verify_standing(a.b, seq, count);
+    const uint32_t r = a.accepted[seq], count = a.b.counts ? min(a.b.counts[seq], a.b.drafts) : a.b.drafts;
     const VerifyRow row = verify_row(a.b, seq, r, count);
     // segments, 64 at most: running sums by lane
     const bool mine = lane < a.segments;
@@ -318,61 +401,67 @@ __global__ __launch_bounds__(256) void verify_pick_kernel(VerifyArgs a)
     uint32_t pick = 0;
     if (any) {
         const int seg = over ? __builtin_ctzll(over) : 63 - __builtin_clzll(any);
-        const double before = __shfl(upto - own, seg, 64);
-        const uint32_t j0 = seg * a.length, j1 = min(j0 + a.length, a.b.vocab), each = a.length / 256;
+        double before = __shfl(upto - own, seg, 64);
+        const uint32_t j0 = seg * a.length, j1 = min(j0 + a.length, a.b.vocab);
         if (threadIdx.x == 0) {
             found = 0xffffffffu;
             last = 0;
         }
-        auto weight = [&](uint32_t j) {
-            const float p = row.p[j];
-            return use_rest ? verify_rest(row, j, p, row.q ? row.q[j] : 0.f) : verify_whole(p);
-        };
-        const uint32_t from = j0 + threadIdx.x * each, to = min(from + each, j1);
-        double sum = 0.0;
-        uint32_t some = 0xffffffffu;
-        for (uint32_t j = from; j < to; j++) {
-            const double w = weight(j);
-            sum += w;
-            if (w > 0.0) some = j;
-        }
-        double run = sum;
+        // 2048 entries at a time, eight neighbours a thread, until the running sum passes the goal; the last entry that holds something is the way out
+        for (uint32_t k0 = j0; k0 < j1; k0 += 2048) {
+            const uint32_t from = k0 + threadIdx.x * 8;
+            double w[8], sum = 0.0;
+            uint32_t some = 0xffffffffu;
 #pragma unroll
-        for (int off = 1; off < 64; off <<= 1) {
-            const double v = __shfl_up(run, off, 64);
-            if (lane >= (uint32_t)off) run += v;
-        }
-        if (lane == 63) waves[wave] = run;
-        __syncthreads();
-        double start = before;
-        for (uint32_t w = 0; w < wave; w++) start += waves[w];
-        run += start;
-        // the first thread whose sums pass the goal looks for the place; the last one that holds something is the way out
-        const bool passes = run > goal && sum > 0.0;
-        const uint64_t first = __ballot(passes), holds = __ballot(some != 0xffffffffu);
-        if (first && lane == (uint32_t)__builtin_ctzll(first)) {
-            double at = run - sum;
-            uint32_t j = from;
-            uint32_t best = some;
-            for (; j < to; j++) {
-                const double w = weight(j);
-                at += w;
-                if (w > 0.0 && at > goal) {
-                    best = j;
-                    break;
-                }
+            for (uint32_t h = 0; h < 2; h++) {
+                float p[4], q[4];
+                verify_load4(row, min(from + 4 * h, j1), j1, p, q);
+#pragma unroll
+                for (uint32_t e = 0; e < 4; e++) w[4 * h + e] = use_rest ? verify_rest(row.x, from + 4 * h + e, p[e], q[e]) : verify_whole(p[e]);
             }
-            atomicMin(&found, best);
+#pragma unroll
+            for (uint32_t e = 0; e < 8; e++) {
+                sum += w[e];
+                some = w[e] > 0.0 ? from + e : some;
+            }
+            double run = sum;
+#pragma unroll
+            for (int off = 1; off < 64; off <<= 1) {
+                const double v = __shfl_up(run, off, 64);
+                if (lane >= (uint32_t)off) run += v;
+            }
+            if (lane == 63) waves[wave] = run;
+            __syncthreads();
+            double start = before;
+            for (uint32_t v = 0; v < wave; v++) start += waves[v];
+            const double all = before + ((waves[0] + waves[1]) + (waves[2] + waves[3]));
+            run += start;
+            const uint64_t first = __ballot((run > goal) & (sum > 0.0)), holds = __ballot(some != 0xffffffffu);
+            if (first && lane == (uint32_t)__builtin_ctzll(first)) {
+                double at = run - sum;
+                uint32_t best = some;
+                bool open = true;
+#pragma unroll
+                for (uint32_t e = 0; e < 8; e++) {
+                    at += w[e];
+                    const bool here = open & (w[e] > 0.0) & (at > goal);
+                    best = here ? from + e : best;
+                    open = here ? false : open;
+                }
+                atomicMin(&found, best);
+            }
+            if (holds && lane == (uint32_t)(63 - __builtin_clzll(holds))) atomicMax(&last, some);
+            __syncthreads();
+            before = all;
+            if (found != 0xffffffffu) break;      // the same in all threads
+            __syncthreads();                      // before `waves` is written again
         }
-        if (holds && lane == (uint32_t)(63 - __builtin_clzll(holds))) atomicMax(&last, some);
-        __syncthreads();
         pick = found != 0xffffffffu ? found : last;
     }
-    if (threadIdx.x <= a.b.drafts && threadIdx.x < 65) {
+    if (threadIdx.x <= a.b.drafts) {
         const uint32_t i = threadIdx.x;
         a.tokens[(uint64_t)seq * (a.b.drafts + 1) + i] = i < r ? a.b.tokens[(uint64_t)seq * a.b.drafts + i] : i == r ? pick : (uint32_t)LV_NO_TOKEN;
     }
-    if (threadIdx.x == 0) a.accepted[seq] = r;
 }
 
 }  // namespace lv

@@ -83,9 +83,12 @@ static int paged_copy(const char *name, bool write, lv_ctx *c, const lv_paged_ca
     a.type = type;
     DeviceScope scope(ctx_device(c));
     HIP_TRY(scope.error);
-    const dim3 grid(batch->tokens, (2 * cache->kv_heads * (cache->dim / 8) + 255) / 256);
-    if (write) paged_copy_kernel<true><<<grid, dim3(256), 0, ctx_stream(c)>>>(a);
-    else paged_copy_kernel<false><<<grid, dim3(256), 0, ctx_stream(c)>>>(a);
+    // tokens a workgroup: as many as 1024 units hold, but no fewer workgroups than there are compute units
+    const uint32_t units = 2 * cache->kv_heads * (cache->dim / 8), room = std::max(1u, std::min(kCopyRun, 256 * kCopyUnits / units));
+    const uint32_t run = std::max(1u, std::min(room, batch->tokens / ctx_units(c)));
+    const dim3 grid((batch->tokens + run - 1) / run, (units + 256 * kCopyUnits - 1) / (256 * kCopyUnits));
+    if (write) paged_copy_kernel<true><<<grid, dim3(256), 0, ctx_stream(c)>>>(a, run);
+    else paged_copy_kernel<false><<<grid, dim3(256), 0, ctx_stream(c)>>>(a, run);
     HIP_TRY(hipGetLastError());
     return LV_OK;
 }
