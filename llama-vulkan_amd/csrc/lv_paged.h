@@ -720,6 +720,7 @@ __global__ __launch_bounds__(256, paged_rows_waves(D, CT, NQ, QT)) void paged_ro
 // The running maximum is a reference that follows the true one when that is 2^8 above it, so that most tiles do not rescale.
 // Weights enter the second product as one fp16 (2^-11) or bf16 (2^-8) number: beside a 16-bit result's own rounding, over all the keys of a row.
 typedef float pg_f16v __attribute__((ext_vector_type(16)));
+typedef uint32_t pg_u4 __attribute__((ext_vector_type(4)));
 
 template <bool BF> __device__ __forceinline__ pg_f16v pg_mfma32(typename PgFrag<BF>::type a, typename PgFrag<BF>::type b, pg_f16v c)
 {
@@ -727,8 +728,15 @@ template <bool BF> __device__ __forceinline__ pg_f16v pg_mfma32(typename PgFrag<
     else return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
 }
 
-typedef const __attribute__((address_space(1))) void pg_glb;
 typedef __attribute__((address_space(3))) void pg_lds;
+
+// 64 x 16 bytes from base + each lane's offset to LDS, lane after lane from `to` on.  The compiler would let every read of LDS wait for all direct loads that it knows
+// of, and so for the tile after the one that is read; the loop's own wait, for the tile it is about to read, is all that is needed.  (2048 tokens behind 6144: 279 us
+// with the builtin, 313 through registers, 2?? so.)  Nothing of a register is written, so nothing can be in flight behind the compiler's back but LDS that it is not to read yet.
+__device__ __forceinline__ void pg_load_direct(uint32_t to, const uint8_t *base, uint32_t offset)
+{
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" : : "s"(__builtin_amdgcn_readfirstlane(to)), "v"(offset), "s"(base) : "memory");
+}
 
 constexpr int kPagedTileRows = 128;
 constexpr float paged_tile_lift(bool bf) { return bf ? 0.f : 6.f; }      // weights up to 2^(6 + 8) in fp16
@@ -739,11 +747,13 @@ __global__ __launch_bounds__(256, 2) void paged_tile_kernel(PagedAttnArgs a)
     constexpr int KS = D / 16, DT = D / 32, CH = D / 8, ROW = 2 * D, STAGE = 2 * 64 * ROW, SLOW = 8;
     constexpr float kLift = paged_tile_lift(BF);
     typedef typename PgFrag<BF>::type Frag;
-    __shared__ __attribute__((aligned(1024))) uint8_t lds[2 * STAGE];      // stage: 64 rows of keys, 64 of values
+    __shared__ __attribute__((aligned(128))) uint8_t lds[2 * STAGE];      // stage: 64 rows of keys, 64 of values
+    __shared__ uint32_t special;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l32 = lane & 31, hh = lane >> 5;
     const uint32_t head = blockIdx.x % a.c.kv_heads, item = blockIdx.x / a.c.kv_heads;
     const PagedItem it = paged_locate<false>(a, item, lane);
     if (!it.any) return;
+    if (threadIdx.x == 0) special = 0;      // ordered by the loop's barriers, and the one behind it
     const uint32_t group = a.deal.group, rows = it.s.rows * group, r0 = it.tile * kPagedTileRows, psize = 1u << a.c.shift;
 
     // keys that rows first .. last see, any of them and all of them
@@ -771,15 +781,21 @@ __global__ __launch_bounds__(256, 2) void paged_tile_kernel(PagedAttnArgs a)
     // a wave brings 16 keys and their values, which lie in one page.  Chunks of 16 bytes are stored at places that depend on their row: keys are read by 32 rows at
     // once (chunk ^ row % 16), values by 4 rows x 64 bytes (groups of four chunks ^ row % 4; of two rows in 256 bytes, ^ half the row)
     constexpr int PER = 64 / CH, LOADS = 16 / PER;      // rows a load, loads
+    // what a lane brings of keys by its load i, and of values: places in the wave's 16 rows
+    uint32_t key_at[LOADS];
+#pragma unroll
+    for (int i = 0; i < LOADS; i++) {
+        const int row = i * PER + lane / CH;
+        key_at[i] = (uint32_t)(row * ROW + ((lane % CH) ^ (row % (CH < 16 ? CH : 16))) * 16);
+    }
+    const uint32_t value_row = lane / CH, value_at = value_row * ROW + ((lane % CH) ^ (CH == 8 ? (value_row / 2 % 2) * 4 : (value_row % 4) * 4)) * 16;
     auto issue = [&](int st, uint32_t page, uint32_t in) {
         const uint8_t *keys = a.c.data + ((uint64_t)(page != kNoPage ? page : 0) * a.c.kv_heads + head) * a.c.block + in * ROW, *vals = keys + a.c.half;
-        uint8_t *kd = lds + st * STAGE + wave * (16 * ROW), *vd = kd + 64 * ROW;
+        const uint32_t kd = (uint32_t)(uintptr_t)(pg_lds *)(lds + st * STAGE + wave * (16 * ROW));
 #pragma unroll
         for (int i = 0; i < LOADS; i++) {
-            const int row = i * PER + lane / CH, ch = lane % CH;
-            const int kx = row % (CH < 16 ? CH : 16), vx = CH == 8 ? (row / 2 % 2) * 4 : (row % 4) * 4;
-            __builtin_amdgcn_global_load_lds((pg_glb *)(keys + (uint32_t)(row * ROW + (ch ^ kx) * 16)), (pg_lds *)(kd + i * 1024), 16, 0, 0);
-            __builtin_amdgcn_global_load_lds((pg_glb *)(vals + (uint32_t)(row * ROW + (ch ^ vx) * 16)), (pg_lds *)(vd + i * 1024), 16, 0, 0);
+            pg_load_direct(kd + i * 1024, keys, key_at[i]);
+            pg_load_direct(kd + 64 * ROW + i * 1024, vals + i * 1024, value_at);      // rows differ by multiples of 4 from load to load
         }
     };
     auto page_of = [&](uint32_t at) { return paged_page_uniform(a, table, at); };
@@ -827,6 +843,42 @@ __global__ __launch_bounds__(256, 2) void paged_tile_kernel(PagedAttnArgs a)
         for (int i = 0; i < 16; i++) o[d][i] = 0.f;
     float m = -1e30f, l = 0.f;
 
+    // which of a tile's four runs of 16 keys have a page
+    auto pages_of = [&](uint32_t kb) {
+        uint32_t ok = 0;
+#pragma unroll
+        for (int g = 0; g < 4; g++) ok |= (page_of(kb + 16 * g) != kNoPage ? 1u : 0u) << g;
+        return ok;
+    };
+    // does some row of the workgroup not see some key of a tile?
+    auto partly = [&](uint32_t kb, uint32_t ok) { return kb < all.all_lo || kb + 64 > all.all_hi || ok != 15; };
+    // In such a tile values that no row sees become 0 (0 times what earlier users of a page left there has to be 0), and so do numbers that are not finite, which
+    // are added behind the loop to the rows that see them.
+    auto clean = [&](uint8_t *vals, uint32_t kb, uint32_t ok) {
+        uint32_t odd = 0;
+        for (int c = threadIdx.x; c < 64 * CH; c += 256) {
+            const uint32_t row = c / CH;
+            pg_u4 *w = reinterpret_cast<pg_u4 *>(vals + c * 16), x = *w;
+            if (kb + row - all.lo < ((ok >> (row / 16)) & 1 ? all.hi - all.lo : 0u)) {
+                const uint32_t here = pg_special<BF>(x[0]) | pg_special<BF>(x[1]) | pg_special<BF>(x[2]) | pg_special<BF>(x[3]);
+                if (here) *w = __builtin_bit_cast(pg_u4, pg_only<BF>(__builtin_bit_cast(Frag, x), 0));
+                odd |= here;
+            } else {
+                *w = pg_u4{0, 0, 0, 0};
+            }
+        }
+        if (odd) special = 1;
+        __syncthreads();
+    };
+    // values of 16 keys as the first operand for 32 dimensions: a lane has dimension l32, keys 4 hh .. + 3 and 8 + 4 hh .. + 3
+    const int vrow = 4 * hh + (lane & 15) / 4, vx = CH == 8 ? (vrow / 2 % 2) * 4 : (vrow % 4) * 4, vch = (l32 / 16) * 2 + (lane & 3) / 2, voff = (lane & 1) * 8;
+    auto values = [&](const uint8_t *vals, int d, int j) {
+        const uint8_t *at = vals + (16 * j + vrow) * ROW + ((4 * d + vch) ^ vx) * 16 + voff;
+        const pg_s4 u = pg_read_columns(at), v = pg_read_columns(at + 8 * ROW);
+        return __builtin_bit_cast(Frag, pg_s8{u[0], u[1], u[2], u[3], v[0], v[1], v[2], v[3]});
+    };
+
+    const uint32_t t_first = t;
     int st = 0;
     for (; t < t_end; t++, st ^= 1) {
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -835,41 +887,28 @@ __global__ __launch_bounds__(256, 2) void paged_tile_kernel(PagedAttnArgs a)
             issue(st ^ 1, mine, (base + (t + 1) * 64 + wave * 16) & (psize - 1));
             if (t + 2 < t_end) mine = page_of(base + (t + 2) * 64 + wave * 16);
         }
-        const uint32_t kb = base + t * 64;
-        uint32_t ok = 0;      // of 16 keys each: is there a page?
-#pragma unroll
-        for (int g = 0; g < 4; g++) ok |= (page_of(kb + 16 * g) != kNoPage ? 1u : 0u) << g;
+        const uint32_t kb = base + t * 64, ok = pages_of(kb);
         uint8_t *kt_lds = lds + st * STAGE, *vt_lds = kt_lds + 64 * ROW;
-        int special = 0;
-        if (kb < all.all_lo || kb + 64 > all.all_hi || ok != 15) {
-            // some row does not see some key: values that no row sees become 0, and others are looked through for numbers that are not finite
-            uint32_t odd = 0;
-            for (int c = threadIdx.x; c < 64 * CH; c += 256) {
-                const uint32_t row = c / CH;
-                uint4 *w = reinterpret_cast<uint4 *>(vt_lds + c * 16);
-                if (kb + row - all.lo < ((ok >> (row / 16)) & 1 ? all.hi - all.lo : 0u)) odd |= pg_special<BF>(w->x) | pg_special<BF>(w->y) | pg_special<BF>(w->z) | pg_special<BF>(w->w);
-                else *w = make_uint4(0, 0, 0, 0);
-            }
-            special = __syncthreads_or(odd != 0);
-        }
+        if (partly(kb, ok)) clean(vt_lds, kb, ok);
         if (idle || kb >= own.hi || kb + 64 <= own.lo) continue;
         const bool edge = kb < own.all_lo || kb + 64 > own.all_hi || ok != 15;
 
         pg_f16v sc[2];
 #pragma unroll
-        for (int kt = 0; kt < 2; kt++) {
+        for (int kt = 0; kt < 2; kt++)
 #pragma unroll
             for (int i = 0; i < 16; i++) sc[kt][i] = 0.f;
 #pragma unroll
-            for (int k = 0; k < KS; k++) {
+        for (int k = 0; k < KS; k++)
+#pragma unroll
+            for (int kt = 0; kt < 2; kt++) {
                 const int row = kt * 32 + l32;
                 const Frag f = *reinterpret_cast<const Frag *>(kt_lds + row * ROW + ((2 * k + hh) ^ (row % (CH < 16 ? CH : 16))) * 16);
                 sc[kt] = pg_mfma32<BF>(f, q[k], sc[kt]);
             }
-        }
         // score i of kt is key 32 kt + 8 (i / 4) + 4 hh + i % 4
-        const uint32_t first = kb + 4 * hh - lo;
         if (edge) {
+            const uint32_t first = kb + 4 * hh - lo;
 #pragma unroll
             for (int kt = 0; kt < 2; kt++)
 #pragma unroll
@@ -906,15 +945,21 @@ __global__ __launch_bounds__(256, 2) void paged_tile_kernel(PagedAttnArgs a)
                 else p[j][e] = (_Float16)w;
             }
         l += sum;
-        // values of 16 keys as the first operand for 32 dimensions: lane has dimension l32, keys 4 hh .. + 3 and 8 + 4 hh .. + 3
-        const int vrow = 4 * hh + (lane & 15) / 4, vx = CH == 8 ? (vrow / 2 % 2) * 4 : (vrow % 4) * 4, vch = (l32 / 16) * 2 + (lane & 3) / 2, voff = (lane & 1) * 8;
-        auto values = [&](int d, int j) {
-            const uint8_t *at = vt_lds + (16 * j + vrow) * ROW + ((4 * d + vch) ^ vx) * 16 + voff;
-            const pg_s4 u = pg_read_columns(at), v = pg_read_columns(at + 8 * ROW);
-            return __builtin_bit_cast(Frag, pg_s8{u[0], u[1], u[2], u[3], v[0], v[1], v[2], v[3]});
-        };
-        if (special) {
-            // kinds 1 to 3, NaN, inf and -inf: their counts among the keys that a row sees
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+#pragma unroll
+            for (int d = 0; d < DT; d++) o[d] = pg_mfma32<BF>(values(vt_lds, d, j), p[j], o[d]);
+    }
+    __syncthreads();
+    if (special) {
+        // kinds 1 to 3, NaN, inf and -inf: their counts among the keys that a row sees, as a product of ones
+        for (t = t_first; t < t_end; t++) {
+            const uint32_t kb = base + t * 64, ok = pages_of(kb);
+            if (!partly(kb, ok)) continue;
+            issue(0, page_of(kb + wave * 16), (kb + wave * 16) & (psize - 1));
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            __syncthreads();
+#pragma unroll 1
             for (int kind = 1; kind <= 3; kind++) {
                 const float add = kind == 1 ? __builtin_nanf("") : kind == 2 ? INFINITY : -INFINITY;
 #pragma unroll
@@ -926,25 +971,18 @@ __global__ __launch_bounds__(256, 2) void paged_tile_kernel(PagedAttnArgs a)
                         Frag one;
 #pragma unroll
                         for (int e = 0; e < 8; e++) {
-                            const float w = first + (16 * j + 8 * (e / 4) + e % 4) < ((ok >> j) & 1 ? span : 0u) ? 1.f : 0.f;
+                            const float w = kb + 4 * hh - lo + (16 * j + 8 * (e / 4) + e % 4) < ((ok >> j) & 1 ? span : 0u) ? 1.f : 0.f;
                             if constexpr (BF) one[e] = (__bf16)w;
                             else one[e] = (_Float16)w;
                         }
-                        n = pg_mfma32<BF>(pg_only<BF>(values(d, j), kind), one, n);
+                        n = pg_mfma32<BF>(pg_only<BF>(values(lds + 64 * ROW, d, j), kind), one, n);
                     }
 #pragma unroll
                     for (int i = 0; i < 16; i++) o[d][i] += n[i] > 0.f ? add : 0.f;
                 }
             }
+            __syncthreads();
         }
-#pragma unroll
-        for (int d = 0; d < DT; d++)
-#pragma unroll
-            for (int j = 0; j < 4; j++) {
-                Frag v = values(d, j);
-                if (special) v = pg_only<BF>(v, 0);
-                o[d] = pg_mfma32<BF>(v, p[j], o[d]);
-            }
     }
 
     l += __shfl_xor(l, 32, 64);
