@@ -19,6 +19,7 @@ typedef _Float16 pg_h8 __attribute__((ext_vector_type(8)));
 typedef _Float16 pg_h2 __attribute__((ext_vector_type(2)));
 typedef __bf16 pg_b8 __attribute__((ext_vector_type(8)));
 typedef float pg_f4 __attribute__((ext_vector_type(4)));
+typedef uint32_t pg_u4 __attribute__((ext_vector_type(4)));      // where uint4, a class, would be kept in memory
 typedef short pg_s4 __attribute__((ext_vector_type(4)));
 typedef short pg_s8 __attribute__((ext_vector_type(8)));
 
@@ -34,6 +35,7 @@ struct PagedAttnArgs {
     uint32_t ldq, ldo, type;
     float scale;                // times log2 e
     const float *sinks;
+    uint32_t round;             // items of a key head that the device's compute units take at once, or 0
     float *part, *part_ml;      // of cut items: [item][kv head][tile][dim], [item][kv head][tile][2]
 };
 
@@ -71,36 +73,39 @@ __device__ __forceinline__ PagedSeq paged_seq_of(const PagedAttnArgs &a, uint32_
     return paged_seq(a.starts[b], a.starts[b + 1], a.lens[b], a.deal.tokens, a.deal.positions);
 }
 
-// steps of all tiles of all sequences: the same sum in every wave of both launches
-__device__ __forceinline__ float paged_all_steps(const PagedAttnArgs &a, int lane)
-{
-    float sum = 0.f;
-    for (uint32_t b0 = 0; b0 < a.deal.seqs; b0 += 64) {
-        float steps = 0.f;
-        if (b0 + lane < a.deal.seqs) {
-            const PagedSeq s = paged_seq_of(a, b0 + lane);
-            steps = (float)paged_tiles(a.deal, s) * (float)paged_steps(a.deal, s);
-        }
-        sum += wave_sum(steps);
-    }
-    return sum;
-}
-
-// The sequence that an item (BY_ROW false) or a row of the tensors (true; `sub`: which of the heads that share a key head) belongs to, found by each wave on its own.
+// The sequence that an item (BY_ROW false) or a row of the tensors (true; `sub`: which of the heads that share a key head) belongs to, found by each wave on its own.  The run
+// follows from the steps of all tiles of all sequences, summed up in the same order by every wave of both launches.
 template <bool BY_ROW> __device__ __forceinline__ PagedItem paged_locate(const PagedAttnArgs &a, uint32_t which, int lane, uint32_t sub = 0)
 {
     PagedItem it{};
-    it.run = __builtin_amdgcn_readfirstlane(paged_run(a.deal, a.deal.target ? paged_all_steps(a, lane) : 0.f));
-    uint32_t before = 0;
-    for (uint32_t b0 = 0; b0 < a.deal.seqs; b0 += 64) {
-        PagedSeq s{};
-        uint32_t tiles = 0, parts = 1;
-        if (b0 + lane < a.deal.seqs) {
-            s = paged_seq_of(a, b0 + lane);
+    PagedSeq s{};
+    uint32_t tiles = 0, steps = 1;
+    auto look = [&](uint32_t b) {
+        s = PagedSeq{};
+        tiles = 0;
+        steps = 1;
+        if (b < a.deal.seqs) {
+            s = paged_seq_of(a, b);
             tiles = paged_tiles(a.deal, s);
-            parts = paged_parts(paged_steps(a.deal, s), it.run);
+            steps = paged_steps(a.deal, s);
         }
-        const uint32_t upto = before + wave_running_sum_u32(tiles * parts);
+    };
+    float all = 0.f;
+    look(lane);
+    if (a.deal.target) {
+        all = wave_sum((float)tiles * (float)steps);
+        if (a.deal.seqs > 64) {
+            for (uint32_t b0 = 64; b0 < a.deal.seqs; b0 += 64) {
+                look(b0 + lane);
+                all += wave_sum((float)tiles * (float)steps);
+            }
+            look(lane);
+        }
+    }
+    it.run = __builtin_amdgcn_readfirstlane(paged_run(a.deal, all));
+    uint32_t before = 0;
+    for (uint32_t b0 = 0;;) {
+        const uint32_t parts = paged_parts(steps, it.run), upto = before + wave_running_sum_u32(tiles * parts);
         const uint64_t here = __ballot(BY_ROW ? which >= s.row0 && which - s.row0 < s.rows : upto > which);
         if (here) {
             const int l = __builtin_ctzll(here);
@@ -121,8 +126,10 @@ template <bool BY_ROW> __device__ __forceinline__ PagedItem paged_locate(const P
             return it;
         }
         before = __builtin_amdgcn_readlane(upto, 63);
+        b0 += 64;
+        if (b0 >= a.deal.seqs) return it;
+        look(b0 + lane);
     }
-    return it;
 }
 
 // ---- elements ----------------------------------------------------------------------------------------------------------------------
@@ -169,34 +176,35 @@ __device__ __forceinline__ void pg_store8(void *p, uint32_t type, uint64_t at, c
     }
     *reinterpret_cast<uint4 *>(static_cast<uint16_t *>(p) + at) = type == LV_F16 ? pg_pack8<false>(x) : pg_pack8<true>(x);
 }
-// N times eight elements, eight of them every `step`: all loads before the first use
-template <int N> __device__ __forceinline__ void pg_load_row(const void *p, uint32_t type, uint64_t at, uint32_t step, float (&x)[N][8])
+// N times eight elements, eight of them every `step`: asked for, and made numbers of later
+template <int N> struct PgRow {
+    pg_u4 u[N], v[N];
+};
+// WIDE: may they have 32 bits?
+template <bool WIDE, int N> __device__ __forceinline__ void pg_ask_row(const void *p, uint32_t type, uint64_t at, uint32_t step, PgRow<N> &r)
 {
-    uint4 u[N], v[N];
-    if (type == LV_F32) {
-        const uint4 *f = reinterpret_cast<const uint4 *>(static_cast<const float *>(p) + at);
+    const uint32_t size = WIDE && type == LV_F32 ? 4 : 2;
+    const uint8_t *f = static_cast<const uint8_t *>(p) + at * size;
 #pragma unroll
-        for (int n = 0; n < N; n++) {
-            u[n] = f[n * (step / 4)];
-            v[n] = f[n * (step / 4) + 1];
-        }
-#pragma unroll
-        for (int n = 0; n < N; n++) {
-            const uint32_t w[8] = {u[n].x, u[n].y, u[n].z, u[n].w, v[n].x, v[n].y, v[n].z, v[n].w};
-#pragma unroll
-            for (int e = 0; e < 8; e++) x[n][e] = __uint_as_float(w[e]);
-        }
-        return;
+    for (int n = 0; n < N; n++) {
+        r.u[n] = *reinterpret_cast<const pg_u4 *>(f + n * step * size);
+        if constexpr (WIDE) r.v[n] = *reinterpret_cast<const pg_u4 *>(f + n * step * size + (size == 4 ? 16 : 0));
     }
-    const uint4 *h = reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(p) + at);
+}
+template <bool WIDE, int N> __device__ __forceinline__ void pg_row_numbers(uint32_t type, const PgRow<N> &r, float (&x)[N][8])
+{
+    if (WIDE && type == LV_F32) {
 #pragma unroll
-    for (int n = 0; n < N; n++) u[n] = h[n * (step / 8)];
-    if (type == LV_F16) {
+        for (int n = 0; n < N; n++) {
+            #pragma unroll
+            for (int e = 0; e < 8; e++) x[n][e] = __uint_as_float(e < 4 ? r.u[n][e % 4] : r.v[n][e % 4]);
+        }
+    } else if (type == LV_F16) {
 #pragma unroll
-        for (int n = 0; n < N; n++) pg_unpack8<false>(u[n], x[n]);
+        for (int n = 0; n < N; n++) pg_unpack8<false>(__builtin_bit_cast(uint4, r.u[n]), x[n]);
     } else {
 #pragma unroll
-        for (int n = 0; n < N; n++) pg_unpack8<true>(u[n], x[n]);
+        for (int n = 0; n < N; n++) pg_unpack8<true>(__builtin_bit_cast(uint4, r.u[n]), x[n]);
     }
 }
 
@@ -276,6 +284,7 @@ __device__ __forceinline__ pg_s4 pg_read_columns(const uint8_t *p)
 constexpr int paged_rows_waves(int D, int CT, int NQ, int QT)
 {
     if (D == 256) return 1;
+    if (D == 128 && QT == 2 && NQ == 3) return 1;      // 59 registers in memory cost more than a second wave gains (1024 tokens behind 3072: 340 us and 281)
     if (D == 128) return QT == 1 && NQ == 1 && CT >= kPgQ8 ? 3 : 2;
     return NQ > 1 && QT == 2 ? 2 : 3;
 }
@@ -298,50 +307,22 @@ __global__ __launch_bounds__(256, paged_rows_waves(D, CT, NQ, QT)) void paged_ro
     const uint32_t group = a.deal.group, rows = it.s.rows * group, r0 = it.tile * TILE;
     const uint32_t psize = 1u << a.c.shift;
 
-    // this lane's rows
-    Frag q[QT][KS][NQ];
-    float factor[QT];
+    // this lane's rows: asked for here, made operands of when the first keys and values are on their way too
+    constexpr int QS = CT == kPgQ4 ? 2 * KS : KS;
+    PgRow<QS> raw[QT];
     uint32_t lo[QT], span[QT];      // the keys it sees: lo .. lo + span - 1
 #pragma unroll
     for (int i = 0; i < QT; i++) {
         const uint32_t r = r0 + i * 16 + l16;
-        const bool mine = r < rows;
-        const uint32_t t = mine ? r / group : 0, h = head * group + (mine ? r - t * group : 0);
-        const int32_t p = it.s.pos0 + (int32_t)t;
+        const bool is = r < rows;
+        const uint32_t tk = is ? r / group : 0, h = head * group + (is ? r - tk * group : 0);
+        const int32_t p = it.s.pos0 + (int32_t)tk;
         lo[i] = p >= 0 ? paged_first_key((uint32_t)p, a.deal.window, a.deal.chunk) : 0;
         const uint32_t end = p >= 0 ? min((uint32_t)p + 1, it.s.keys) : 0;
-        span[i] = mine && end > lo[i] ? end - lo[i] : 0;
-        float z[KS][8], top = 0.f;
-        const uint64_t at = (uint64_t)(it.s.row0 + t) * a.ldq + (uint64_t)h * D;
-        if constexpr (CT == kPgQ4) {      // byte 4 g + j of a block holds elements 4 g + j and 16 + 4 g + j
-            float u[2 * KS][8];
-            pg_load_row<2 * KS>(a.q, a.type, at + (g4 / 2) * 8, 16, u);
-#pragma unroll
-            for (int k = 0; k < KS; k++)
-#pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    const float a0 = u[2 * k][e], a1 = u[2 * k][4 + e], b0 = u[2 * k + 1][e], b1 = u[2 * k + 1][4 + e];
-                    z[k][e] = g4 & 1 ? a1 : a0;
-                    z[k][4 + e] = g4 & 1 ? b1 : b0;
-                }
-        } else {
-            pg_load_row<KS>(a.q, a.type, at + g4 * 8, 32, z);
-        }
-#pragma unroll
-        for (int k = 0; k < KS; k++)
-#pragma unroll
-            for (int e = 0; e < 8; e++) top = fmaxf(top, fabsf(z[k][e]));
-        top = fmaxf(top, __shfl_xor(top, 16, 64));
-        top = fmaxf(top, __shfl_xor(top, 32, 64));
-        // a power of two brings the row's largest element to 2^10 .. 2^11: no overflow, and small pieces are no subnormals
-        int e2 = (int)(__float_as_uint(top) >> 23) - 127 - 10;
-        if (e2 > 117 || e2 < -110) e2 = 0;      // inf, NaN; 0 and numbers next to it
-        const float down = __uint_as_float((uint32_t)(127 - e2) << 23);
-        factor[i] = a.scale * __uint_as_float((uint32_t)(127 + e2) << 23);
-#pragma unroll
-        for (int k = 0; k < KS; k++)
-#pragma unroll
-            for (int e = 0; e < 8; e++) pg_cut<BF, NQ>(mine ? z[k][e] * down : 0.f, e, q[i][k]);
+        span[i] = is && end > lo[i] ? end - lo[i] : 0;
+        const uint64_t at = (uint64_t)(it.s.row0 + tk) * a.ldq + (uint64_t)h * D;
+        if constexpr (CT == kPgQ4) pg_ask_row<EXACT, QS>(a.q, a.type, at + (g4 / 2) * 8, 16, raw[i]);
+        else pg_ask_row<EXACT, QS>(a.q, a.type, at + g4 * 8, 32, raw[i]);
     }
     // keys that any row sees, and those that all rows see
     const uint32_t last_row = min(r0 + TILE, rows) - 1;
@@ -350,7 +331,7 @@ __global__ __launch_bounds__(256, paged_rows_waves(D, CT, NQ, QT)) void paged_ro
     const uint32_t k_hi = p_last >= 0 ? min((uint32_t)p_last + 1, it.s.keys) : 0;
     const uint32_t all_lo = p_last >= 0 ? paged_first_key((uint32_t)p_last, a.deal.window, a.deal.chunk) : 0, all_hi = p_first >= 0 ? (uint32_t)p_first + 1 : 0;
     const uint32_t base = k_lo & ~31u, n_steps = k_hi > base ? (k_hi - base + kPagedStep - 1) / kPagedStep : 0;
-    const uint32_t s0 = min((uint64_t)it.part * it.run, (uint64_t)n_steps), s1 = min((uint64_t)s0 + it.run, (uint64_t)n_steps);
+    const uint32_t s0 = paged_cut(n_steps, it.part, it.parts), s1 = paged_cut(n_steps, it.part + 1, it.parts);
 
     const uint32_t *table = a.table + (uint64_t)it.seq * a.table_ld;
     const uint32_t turns = n_steps ? (k_hi - base + 31) / 32 : 0, t_end = min(s1 * 4, turns);
@@ -462,6 +443,39 @@ __global__ __launch_bounds__(256, paged_rows_waves(D, CT, NQ, QT)) void paged_ro
         load_keys(page0, page1, in0, in1);
         load_values(page0, page1, in0, in1);
     }
+
+    Frag q[QT][KS][NQ];
+    float factor[QT];
+#pragma unroll
+    for (int i = 0; i < QT; i++) {
+        float u[QS][8], z[KS][8], top = 0.f;
+        pg_row_numbers<EXACT, QS>(a.type, raw[i], u);
+#pragma unroll
+        for (int k = 0; k < KS; k++)
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                if constexpr (CT == kPgQ4) {      // byte 4 g + j of a block holds elements 4 g + j and 16 + 4 g + j
+                    const float a0 = u[2 * k + e / 4][e % 4], a1 = u[2 * k + e / 4][4 + e % 4];
+                    z[k][e] = g4 & 1 ? a1 : a0;
+                } else {
+                    z[k][e] = u[k][e];
+                }
+                top = fmaxf(top, fabsf(z[k][e]));
+            }
+        top = fmaxf(top, __shfl_xor(top, 16, 64));
+        top = fmaxf(top, __shfl_xor(top, 32, 64));
+        // a power of two brings the row's largest element to 2^10 .. 2^11: no overflow, and small pieces are no subnormals
+        int e2 = (int)(__float_as_uint(top) >> 23) - 127 - 10;
+        if (e2 > 117 || e2 < -110) e2 = 0;      // inf, NaN; 0 and numbers next to it
+        const float down = __uint_as_float((uint32_t)(127 - e2) << 23);
+        factor[i] = a.scale * __uint_as_float((uint32_t)(127 + e2) << 23);
+        const bool is = r0 + i * 16 + l16 < rows;
+#pragma unroll
+        for (int k = 0; k < KS; k++)
+#pragma unroll
+            for (int e = 0; e < 8; e++) pg_cut<BF, NQ>(is ? z[k][e] * down : 0.f, e, q[i][k]);
+    }
+
     for (; t < t_end; t += 4) {
         asm volatile("" : "+v"(ln));
         const uint32_t kb = base + t * 32;
@@ -717,10 +731,11 @@ __global__ __launch_bounds__(256, paged_rows_waves(D, CT, NQ, QT)) void paged_ro
 // loads; two workgroups a CU, so that one's softmax fills the other's products.  v_mfma_f32_32x32x16: S^T = K Q^T leaves 32 scores of one row in a lane
 // (and 32 in lane ^ 32), and eight registers in a row are an operand of O^T = V^T P^T whose other one comes through ds_read_b64_tr_b16.
 // A wave reads 32 KB of LDS and issues 32 products of 32 clocks for a tile, its share of the LDS's rate and a SIMD's: bound by both, then by the softmax's vector work.
-// The running maximum is a reference that follows the true one when that is 2^8 above it, so that most tiles do not rescale.
+// The running maximum is a reference: weights are formed with it at once, and only where their sum says that a score is far above it are the maximum taken, the results
+// rescaled and the weights formed anew.  Most tiles do without the maximum's 48 vector instructions (half of them make numbers canonical).
 // Weights enter the second product as one fp16 (2^-11) or bf16 (2^-8) number: beside a 16-bit result's own rounding, over all the keys of a row.
 typedef float pg_f16v __attribute__((ext_vector_type(16)));
-typedef uint32_t pg_u4 __attribute__((ext_vector_type(4)));
+
 
 template <bool BF> __device__ __forceinline__ pg_f16v pg_mfma32(typename PgFrag<BF>::type a, typename PgFrag<BF>::type b, pg_f16v c)
 {
@@ -730,27 +745,39 @@ template <bool BF> __device__ __forceinline__ pg_f16v pg_mfma32(typename PgFrag<
 
 typedef __attribute__((address_space(3))) void pg_lds;
 
-// 64 x 16 bytes from base + each lane's offset to LDS, lane after lane from `to` on.  The compiler would let every read of LDS wait for all direct loads that it knows
-// of, and so for the tile after the one that is read; the loop's own wait, for the tile it is about to read, is all that is needed.  (2048 tokens behind 6144: 279 us
-// with the builtin, 313 through registers, 2?? so.)  Nothing of a register is written, so nothing can be in flight behind the compiler's back but LDS that it is not to read yet.
-__device__ __forceinline__ void pg_load_direct(uint32_t to, const uint8_t *base, uint32_t offset)
+// N runs of 64 x 16 bytes from base + 1024 i + each lane's offset to LDS, lane after lane from to + 1024 i on.  The compiler would let every read of LDS wait for all
+// direct loads that it knows of, and so for the tile after the one that is read; the loop's own wait, for the tile it is about to read, is all that is needed.  (2048
+// tokens behind 6144: 279 us with the builtin, 313 through registers, 261 so.)  No register is written, so what is in flight behind the compiler's back is LDS only, which
+// nobody reads yet.
+template <int N> __device__ __forceinline__ void pg_load_direct(uint32_t to, const uint8_t *base, const uint32_t (&at)[N])
 {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" : : "s"(__builtin_amdgcn_readfirstlane(to)), "v"(offset), "s"(base) : "memory");
+    static_assert(N == 2 || N == 4, "runs");
+    if constexpr (N == 4)
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %5\n\tglobal_load_lds_dwordx4 %2, %5 offset:1024\n\t"
+                     "global_load_lds_dwordx4 %3, %5 offset:2048\n\tglobal_load_lds_dwordx4 %4, %5 offset:3072"
+                     : : "s"(__builtin_amdgcn_readfirstlane(to)), "v"(at[0]), "v"(at[1]), "v"(at[2]), "v"(at[3]), "s"(base) : "memory");
+    else
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %3\n\tglobal_load_lds_dwordx4 %2, %3 offset:1024"
+                     : : "s"(__builtin_amdgcn_readfirstlane(to)), "v"(at[0]), "v"(at[1]), "s"(base) : "memory");
 }
 
 constexpr int kPagedTileRows = 128;
-constexpr float paged_tile_lift(bool bf) { return bf ? 0.f : 6.f; }      // weights up to 2^(6 + 8) in fp16
+constexpr float paged_tile_lift(bool bf) { return bf ? 0.f : 6.f; }      // of the weight of a score at the reference, log2
 
 template <int D, bool BF>
 __global__ __launch_bounds__(256, 2) void paged_tile_kernel(PagedAttnArgs a)
 {
-    constexpr int KS = D / 16, DT = D / 32, CH = D / 8, ROW = 2 * D, STAGE = 2 * 64 * ROW, SLOW = 8;
-    constexpr float kLift = paged_tile_lift(BF);
+    constexpr int KS = D / 16, DT = D / 32, CH = D / 8, ROW = 2 * D, STAGE = 2 * 64 * ROW;
+    constexpr float kLift = paged_tile_lift(BF), MOST = 32768.f;      // of a lane's weights in a tile: each fits fp16
     typedef typename PgFrag<BF>::type Frag;
     __shared__ __attribute__((aligned(128))) uint8_t lds[2 * STAGE];      // stage: 64 rows of keys, 64 of values
     __shared__ uint32_t special;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l32 = lane & 31, hh = lane >> 5;
-    const uint32_t head = blockIdx.x % a.c.kv_heads, item = blockIdx.x / a.c.kv_heads;
+    const uint32_t head = blockIdx.x % a.c.kv_heads;
+    uint32_t item = blockIdx.x / a.c.kv_heads;
+    // Items come with those first that see most.  The second workgroup of a compute unit is one of the next round, taken backwards: the sums of two come out even
+    // (64 tiles of 8 key heads, 512 workgroups at once: 256 to 253 us)
+    if (a.round && item / a.round % 2 && (item / a.round + 1) * a.round <= gridDim.x / a.c.kv_heads) item = item / a.round * a.round + (a.round - 1 - item % a.round);
     const PagedItem it = paged_locate<false>(a, item, lane);
     if (!it.any) return;
     if (threadIdx.x == 0) special = 0;      // ordered by the loop's barriers, and the one behind it
@@ -774,29 +801,26 @@ __global__ __launch_bounds__(256, 2) void paged_tile_kernel(PagedAttnArgs a)
     const bool idle = w0 >= rows;      // no row of this wave: it brings its share of the tiles
     const Range own = range(idle ? r0 : w0, min(w0 + 32, rows) - 1);
     const uint32_t base = all.lo & ~31u, n_steps = all.hi > base ? (all.hi - base + kPagedStep - 1) / kPagedStep : 0;
-    const uint32_t s0 = min((uint64_t)it.part * it.run, (uint64_t)n_steps), s1 = min((uint64_t)s0 + it.run, (uint64_t)n_steps);
+    const uint32_t s0 = paged_cut(n_steps, it.part, it.parts), s1 = paged_cut(n_steps, it.part + 1, it.parts);
     const uint32_t tiles = n_steps ? (all.hi - base + 63) / 64 : 0, t_end = min(s1 * (kPagedStep / 64), tiles);
     const uint32_t *table = a.table + (uint64_t)it.seq * a.table_ld;
 
     // a wave brings 16 keys and their values, which lie in one page.  Chunks of 16 bytes are stored at places that depend on their row: keys are read by 32 rows at
     // once (chunk ^ row % 16), values by 4 rows x 64 bytes (groups of four chunks ^ row % 4; of two rows in 256 bytes, ^ half the row)
     constexpr int PER = 64 / CH, LOADS = 16 / PER;      // rows a load, loads
-    // what a lane brings of keys by its load i, and of values: places in the wave's 16 rows
-    uint32_t key_at[LOADS];
+    // what a lane brings by its load i, less 1024 i: places in the wave's 16 rows
+    uint32_t key_at[LOADS], value_at[LOADS];
 #pragma unroll
     for (int i = 0; i < LOADS; i++) {
-        const int row = i * PER + lane / CH;
-        key_at[i] = (uint32_t)(row * ROW + ((lane % CH) ^ (row % (CH < 16 ? CH : 16))) * 16);
+        const int row = i * PER + lane / CH, ch = lane % CH;
+        key_at[i] = (uint32_t)(lane / CH * ROW + (ch ^ (row % (CH < 16 ? CH : 16))) * 16);
+        value_at[i] = (uint32_t)(lane / CH * ROW + (ch ^ (CH == 8 ? (row / 2 % 2) * 4 : (row % 4) * 4)) * 16);
     }
-    const uint32_t value_row = lane / CH, value_at = value_row * ROW + ((lane % CH) ^ (CH == 8 ? (value_row / 2 % 2) * 4 : (value_row % 4) * 4)) * 16;
     auto issue = [&](int st, uint32_t page, uint32_t in) {
-        const uint8_t *keys = a.c.data + ((uint64_t)(page != kNoPage ? page : 0) * a.c.kv_heads + head) * a.c.block + in * ROW, *vals = keys + a.c.half;
-        const uint32_t kd = (uint32_t)(uintptr_t)(pg_lds *)(lds + st * STAGE + wave * (16 * ROW));
-#pragma unroll
-        for (int i = 0; i < LOADS; i++) {
-            pg_load_direct(kd + i * 1024, keys, key_at[i]);
-            pg_load_direct(kd + 64 * ROW + i * 1024, vals + i * 1024, value_at);      // rows differ by multiples of 4 from load to load
-        }
+        const uint8_t *keys = a.c.data + ((uint64_t)(page != kNoPage ? page : 0) * a.c.kv_heads + head) * a.c.block + in * ROW;
+        const uint32_t to = (uint32_t)(uintptr_t)(pg_lds *)(lds + st * STAGE + wave * (16 * ROW));
+        pg_load_direct(to, keys, key_at);
+        pg_load_direct(to + 64 * ROW, keys + a.c.half, value_at);
     };
     auto page_of = [&](uint32_t at) { return paged_page_uniform(a, table, at); };
     uint32_t t = s0 * (kPagedStep / 64), mine = kNoPage;
@@ -816,7 +840,9 @@ __global__ __launch_bounds__(256, 2) void paged_tile_kernel(PagedAttnArgs a)
         const uint32_t end = p >= 0 ? min((uint32_t)p + 1, it.s.keys) : 0;
         span = is && end > lo ? end - lo : 0;
         float z[KS][8], top = 0.f;
-        pg_load_row<KS>(a.q, a.type, (uint64_t)(it.s.row0 + tk) * a.ldq + (uint64_t)h * D + hh * 8, 16, z);
+        PgRow<KS> raw;
+        pg_ask_row<false, KS>(a.q, a.type, (uint64_t)(it.s.row0 + tk) * a.ldq + (uint64_t)h * D + hh * 8, 16, raw);
+        pg_row_numbers<false, KS>(a.type, raw, z);
 #pragma unroll
         for (int k = 0; k < KS; k++)
 #pragma unroll
@@ -843,10 +869,16 @@ __global__ __launch_bounds__(256, 2) void paged_tile_kernel(PagedAttnArgs a)
         for (int i = 0; i < 16; i++) o[d][i] = 0.f;
     float m = -1e30f, l = 0.f;
 
-    // which of a tile's four runs of 16 keys have a page
+    // Which of a tile's four runs of 16 keys have a page?  All of them, unless one of the item's pages is missing: looked up once.
+    uint32_t missing = 0;
+    {
+        const uint32_t k0 = base + s0 * kPagedStep, k1 = min(base + s1 * kPagedStep, all.hi);
+        for (uint32_t i = (k0 >> a.c.shift) + lane; k0 < k1 && i <= (k1 - 1) >> a.c.shift; i += 64) missing |= i >= a.table_ld || table[i] >= a.c.pages ? 1u : 0u;
+        missing = __any(missing != 0);
+    }
     auto pages_of = [&](uint32_t kb) {
+        if (!missing) return 15u;
         uint32_t ok = 0;
-#pragma unroll
         for (int g = 0; g < 4; g++) ok |= (page_of(kb + 16 * g) != kNoPage ? 1u : 0u) << g;
         return ok;
     };
@@ -883,14 +915,18 @@ __global__ __launch_bounds__(256, 2) void paged_tile_kernel(PagedAttnArgs a)
     for (; t < t_end; t++, st ^= 1) {
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __syncthreads();
-        if (t + 1 < t_end) {
+        auto next = [&]() {
+            if (t + 1 >= t_end) return;
             issue(st ^ 1, mine, (base + (t + 1) * 64 + wave * 16) & (psize - 1));
             if (t + 2 < t_end) mine = page_of(base + (t + 2) * 64 + wave * 16);
-        }
+        };
         const uint32_t kb = base + t * 64, ok = pages_of(kb);
         uint8_t *kt_lds = lds + st * STAGE, *vt_lds = kt_lds + 64 * ROW;
         if (partly(kb, ok)) clean(vt_lds, kb, ok);
-        if (idle || kb >= own.hi || kb + 64 <= own.lo) continue;
+        if (idle || kb >= own.hi || kb + 64 <= own.lo) {
+            next();
+            continue;
+        }
         const bool edge = kb < own.all_lo || kb + 64 > own.all_hi || ok != 15;
 
         pg_f16v sc[2];
@@ -906,6 +942,15 @@ __global__ __launch_bounds__(256, 2) void paged_tile_kernel(PagedAttnArgs a)
                 const Frag f = *reinterpret_cast<const Frag *>(kt_lds + row * ROW + ((2 * k + hh) ^ (row % (CH < 16 ? CH : 16))) * 16);
                 sc[kt] = pg_mfma32<BF>(f, q[k], sc[kt]);
             }
+        // reads four products ahead: left alone the compiler reads a pair, waits and multiplies
+        __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
+#pragma unroll
+        for (int k = 0; k < 2 * KS - 4; k++) {
+            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+        }
+        __builtin_amdgcn_sched_group_barrier(0x008, 4, 0);
+        next();      // its scalar work while the products run
         // score i of kt is key 32 kt + 8 (i / 4) + 4 hh + i % 4
         if (edge) {
             const uint32_t first = kb + 4 * hh - lo;
@@ -917,33 +962,37 @@ __global__ __launch_bounds__(256, 2) void paged_tile_kernel(PagedAttnArgs a)
                     sc[kt][i] = first + (32 * kt + 8 * (i / 4) + i % 4) < sees ? sc[kt][i] : -INFINITY;
                 }
         }
-        float top = -INFINITY;
+        Frag p[4];      // 16 keys each
+        float sum;
+        auto weigh = [&]() {
+            const float less = kLift - m;
+            sum = 0.f;
 #pragma unroll
-        for (int kt = 0; kt < 2; kt++)
+            for (int j = 0; j < 4; j++)
 #pragma unroll
-            for (int i = 0; i < 16; i += 2) top = fmaxf(fmaxf(sc[kt][i], sc[kt][i + 1]), top);
-        top = fmaxf(top, __shfl_xor(top, 32, 64)) * factor;
-        if (__any(top > m + SLOW)) {
-            const float to = fmaxf(top, m), f = pg_exp2(m - to);
+                for (int e = 0; e < 8; e++) {
+                    const float w = pg_exp2(fmaf(sc[j / 2][j % 2 * 8 + e], factor, less));
+                    sum += w;
+                    if constexpr (BF) p[j][e] = (__bf16)w;
+                    else p[j][e] = (_Float16)w;
+                }
+        };
+        weigh();
+        if (__any(!(sum <= MOST))) {      // the reference is too small, as at first; or a score is no number
+            float top = -INFINITY;
+#pragma unroll
+            for (int kt = 0; kt < 2; kt++)
+#pragma unroll
+                for (int i = 0; i < 16; i += 2) top = fmaxf(fmaxf(sc[kt][i], sc[kt][i + 1]), top);
+            const float to = fmaxf(fmaxf(top, __shfl_xor(top, 32, 64)) * factor, m), f = pg_exp2(m - to);
             m = to;
             l *= f;
 #pragma unroll
             for (int d = 0; d < DT; d++)
 #pragma unroll
                 for (int i = 0; i < 16; i++) o[d][i] *= f;
+            weigh();
         }
-        const float less = kLift - m;
-        Frag p[4];      // 16 keys each
-        float sum = 0.f;
-#pragma unroll
-        for (int j = 0; j < 4; j++)
-#pragma unroll
-            for (int e = 0; e < 8; e++) {
-                const float w = pg_exp2(fmaf(sc[j / 2][j % 2 * 8 + e], factor, less));
-                sum += w;
-                if constexpr (BF) p[j][e] = (__bf16)w;
-                else p[j][e] = (_Float16)w;
-            }
         l += sum;
 #pragma unroll
         for (int j = 0; j < 4; j++)
@@ -1031,27 +1080,32 @@ __global__ __launch_bounds__(256, 2) void paged_tile_kernel(PagedAttnArgs a)
         }
 }
 
-// ---- the parts of cut items put together: a workgroup a row ------------------------------------------------------------------------
-template <int D>
+// ---- the parts of cut items put together -------------------------------------------------------------------------------------------
+// WAVES waves a row, 4 / WAVES rows a workgroup: four for few rows, which may have many parts; one where there are many rows and most workgroups find nothing to do.
+template <int D, int WAVES>
 __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttnArgs a, float lift)
 {
     __shared__ float sums[4][D], tops[4][2];
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const uint32_t heads = a.c.kv_heads * a.deal.group, row = blockIdx.x / heads, h = blockIdx.x % heads;
-    const PagedItem it = paged_locate<true>(a, row, lane, h % a.deal.group);
-    if (!it.any || it.parts == 1) return;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), first = wave / WAVES * WAVES;
+    const uint32_t heads = a.c.kv_heads * a.deal.group, n = blockIdx.x * (4 / WAVES) + wave / WAVES, row = n / heads, h = n - row * heads;
+    PagedItem it{};
+    if (row < a.deal.tokens) it = paged_locate<true>(a, row, lane, h % a.deal.group);
+    const bool cut = it.any && it.parts > 1;
+    if constexpr (WAVES == 4) {
+        if (!cut) return;
+    }
     const uint32_t group = a.deal.group, kvh = h / group, r = (row - it.s.row0) * group + h % group, in = r - it.tile * a.deal.tile;
-    // wave w takes parts w, w + 4, ..
+    // of a row's parts a wave takes every WAVES-th
     constexpr int V = D >= 64 ? D / 64 : 1;
     const bool mine = lane * V < D;
     float top = -1e30f, all = 0.f, y[V];
 #pragma unroll
     for (int e = 0; e < V; e++) y[e] = 0.f;
-    for (uint32_t p0 = wave; p0 < it.parts; p0 += 16) {
+    for (uint32_t p0 = wave - first; cut && p0 < it.parts; p0 += 4 * WAVES) {
         float ms[4], ls[4], v[4][V];
 #pragma unroll
         for (int j = 0; j < 4; j++) {
-            const uint32_t p = p0 + 4 * j;
+            const uint32_t p = p0 + WAVES * j;
             const uint64_t at = ((uint64_t)(it.first + min(p, it.parts - 1)) * a.c.kv_heads + kvh) * a.deal.tile + in;
             ms[j] = a.part_ml[2 * at];
             ls[j] = a.part_ml[2 * at + 1];
@@ -1083,24 +1137,26 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttnArgs a, float 
         tops[wave][1] = all;
     }
     __syncthreads();
-    if (threadIdx.x >= D / 8) return;
-    float big = fmaxf(fmaxf(tops[0][0], tops[1][0]), fmaxf(tops[2][0], tops[3][0]));
+    if (!cut || wave != first || lane >= D / 8) return;
+    float big = tops[first][0];
+#pragma unroll
+    for (int w = 1; w < WAVES; w++) big = fmaxf(big, tops[first + w][0]);
     const float sink = a.sinks ? a.sinks[h] * 1.44269504088896341f : -1e30f;
     big = fmaxf(big, sink);
     float total = a.sinks ? pg_exp2(sink - big + lift) : 0.f, z[8];
 #pragma unroll
     for (int e = 0; e < 8; e++) z[e] = 0.f;
 #pragma unroll
-    for (int w = 0; w < 4; w++) {
-        const float g = pg_exp2(tops[w][0] - big);
-        total = fmaf(tops[w][1], g, total);
+    for (int w = 0; w < WAVES; w++) {
+        const float g = pg_exp2(tops[first + w][0] - big);
+        total = fmaf(tops[first + w][1], g, total);
 #pragma unroll
-        for (int e = 0; e < 8; e++) z[e] = fmaf(sums[w][threadIdx.x * 8 + e], g, z[e]);
+        for (int e = 0; e < 8; e++) z[e] = fmaf(sums[first + w][lane * 8 + e], g, z[e]);
     }
     const float f = 1.f / total;
 #pragma unroll
     for (int e = 0; e < 8; e++) z[e] = total == 0.f ? 0.f : z[e] * f;
-    pg_store8(a.out, a.type, (uint64_t)row * a.ldo + (uint64_t)h * D + threadIdx.x * 8, z);
+    pg_store8(a.out, a.type, (uint64_t)row * a.ldo + (uint64_t)h * D + lane * 8, z);
 }
 
 }  // namespace lv

@@ -15,9 +15,10 @@ struct AttnPlan {
     uint64_t items, part_floats, bytes;
 };
 
-// Workgroups that share the work of a call.  
-constexpr uint32_t kTargetPerUnit = 4;
+// Workgroups a compute unit that share the work of a call (lv_paged_plan.h)
+constexpr uint32_t kTargetPerUnit = 2;
 constexpr uint32_t kTileRowsMin = 48;
+constexpr uint32_t kJoinRows = 1024;
 
 AttnPlan attn_plan(uint32_t units, uint32_t type, const lv_paged_cache &c, const lv_paged_batch &b, const lv_paged_attn_spec &s)
 {
@@ -37,8 +38,9 @@ AttnPlan attn_plan(uint32_t units, uint32_t type, const lv_paged_cache &c, const
     d.window = s.window;
     d.chunk = s.chunk;
     d.positions = b.table_ld * c.page;
-    d.target = (tile ? 2 : kTargetPerUnit) * units;
+    d.target = kTargetPerUnit * units;
     if ((uint64_t)b.tokens * group / d.tile * c.kv_heads >= d.target) d.target = 0;
+    p.args.round = units / c.kv_heads;
     p.items = paged_items(d);
     p.part_floats = d.target ? p.items * c.kv_heads * d.tile * c.dim : 0;
     p.bytes = d.target ? (p.part_floats + p.items * c.kv_heads * d.tile * 2) * 4 : 0;
@@ -75,7 +77,10 @@ void launch_attention(const AttnPlan &p, uint32_t grid, hipStream_t st)
     case LV_Q8_0: p.pieces == 1 ? launch_rows<D, kPgQ8, 1>(p, grid, st) : launch_rows<D, kPgQ8, 2>(p, grid, st); break;
     default: p.pieces == 1 ? launch_rows<D, kPgQ4, 1>(p, grid, st) : launch_rows<D, kPgQ4, 2>(p, grid, st); break;
     }
-    if (a.deal.target) paged_join_kernel<D><<<dim3(a.deal.tokens * a.deal.group * a.deal.kv_heads), dim3(256), 0, st>>>(a, lift);
+    if (!a.deal.target) return;
+    const uint32_t rows = a.deal.tokens * a.deal.group * a.deal.kv_heads;
+    if (rows >= kJoinRows) paged_join_kernel<D, 1><<<dim3((rows + 3) / 4), dim3(256), 0, st>>>(a, lift);
+    else paged_join_kernel<D, 4><<<dim3(rows), dim3(256), 0, st>>>(a, lift);
 }
 
 }  // namespace

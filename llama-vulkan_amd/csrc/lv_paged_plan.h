@@ -90,10 +90,11 @@ LV_HD uint32_t paged_first_key(uint32_t position, uint32_t window, uint32_t chun
 
 // ---- how attention is dealt to workgroups --------------------------------------------------------------------------------------------
 // A workgroup takes the queries of one key head in tiles of `tile` rows, a row being a token and one of the `group` heads that share the key head, token
-// by token, and a run of the keys that they see.  Keys are counted in steps of kPagedStep; a sequence whose tiles would walk more than `run` steps is cut into
-// parts of so many, whose results a second launch puts together.  The length of a run follows from all lengths at once: the steps of all tiles shared
-// evenly by as many workgroups as the device holds a few times over (`target`), so that one long sequence among short ones is cut finely and equal ones
-// are not cut at all when there are enough of them.
+// by token, and some of the keys that they see.  Keys are counted in steps of kPagedStep; a tile that walks `run` steps or up to half as many more is one item, a longer one
+// is cut into equal parts of about so many, whose results a second launch puts together.  The run follows from all lengths at once: the steps of all tiles shared
+// evenly by as many workgroups as the device holds (`target`), so that one long sequence among short ones is cut finely and equal ones are not cut at all
+// when there are enough of them.  us, 2 or 4 or 8 workgroups a compute unit: 131072 keys of one sequence 97, 106, 111; drafts of 16 sequences 23, 27, 28; 64 sequences of 4096 to
+// 8190 keys 182 when none is cut, 216 with those above the mean cut into a whole run and a rest.
 constexpr uint32_t kPagedStep = 128;
 constexpr uint32_t kPagedRunMin = 2;
 
@@ -119,8 +120,14 @@ LV_HD uint32_t paged_run(const PagedDeal &d, float all_steps)
     const float run = all_steps * (float)d.kv_heads / (float)d.target;
     return run < (float)kPagedRunMin ? kPagedRunMin : run > 1e9f ? 1000000000u : (uint32_t)run + 1;
 }
-LV_HD uint32_t paged_parts(uint32_t steps, uint32_t run) { return steps <= run ? 1 : (steps + run - 1) / run; }
-// items of a key head at most: parts are no more than steps / run + 1 a tile
+LV_HD uint32_t paged_parts(uint32_t steps, uint32_t run)
+{
+    const uint32_t parts = run > 0x3fffffffu ? 1 : (2 * steps + run) / (2 * run);
+    return parts ? parts : 1;
+}
+// the first of a tile's `steps` that is part p's; its last one's end is p + 1's first
+LV_HD uint32_t paged_cut(uint32_t steps, uint32_t p, uint32_t parts) { return (uint32_t)((uint64_t)steps * p / parts); }
+// items of a key head at most: parts are no more than steps / run + 1 / 2 a tile, or 1
 LV_HD uint64_t paged_items(const PagedDeal &d)
 {
     return (uint64_t)d.target / d.kv_heads + 1 + (uint64_t)d.tokens * d.group / d.tile + (d.seqs < d.tokens ? d.seqs : d.tokens);

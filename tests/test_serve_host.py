@@ -223,7 +223,11 @@ int main()
                     const int32_t p0 = x.pos0 + (int32_t)(t * d.tile / d.group), p1 = x.pos0 + (int32_t)(last / d.group);
                     if (p1 < 0) continue;
                     const uint32_t lo = p0 >= 0 ? lv::paged_first_key(p0, d.window, d.chunk) : 0, hi = std::min((uint32_t)p1 + 1, x.keys), base = lo & ~31u;
-                    if (hi > base && (uint64_t)parts * run * lv::kPagedStep < hi - base) missed++;
+                    // parts follow one another from the first step to the last
+                    const uint32_t n = hi > base ? (hi - base + lv::kPagedStep - 1) / lv::kPagedStep : 0;
+                    if (n > steps || lv::paged_cut(n, 0, parts) != 0 || lv::paged_cut(n, parts, parts) != n) missed++;
+                    for (uint32_t p = 0; p < parts; p++)
+                        if (lv::paged_cut(n, p, parts) > lv::paged_cut(n, p + 1, parts)) missed++;
                 }
             }
             printf("%u %llu %llu %u %u\n", run, (unsigned long long)items, (unsigned long long)lv::paged_items(d), missed, cut);
