@@ -9,6 +9,8 @@
 // as well.  Masked scores are -inf, the running maximum starts at a finite -1e30: a row that sees nothing ends with a sum of 0 and is written as 0.
 #pragma once
 
+#include <type_traits>
+
 #include "lv_common.h"
 #include "lv_device.h"
 #include "lv_paged_plan.h"
@@ -16,10 +18,12 @@
 namespace lv {
 
 typedef _Float16 pg_h8 __attribute__((ext_vector_type(8)));
+typedef _Float16 pg_h4 __attribute__((ext_vector_type(4)));
 typedef _Float16 pg_h2 __attribute__((ext_vector_type(2)));
 typedef __bf16 pg_b8 __attribute__((ext_vector_type(8)));
 typedef float pg_f4 __attribute__((ext_vector_type(4)));
 typedef uint32_t pg_u4 __attribute__((ext_vector_type(4)));      // where uint4, a class, would be kept in memory
+typedef uint32_t pg_u2 __attribute__((ext_vector_type(2)));
 typedef short pg_s4 __attribute__((ext_vector_type(4)));
 typedef short pg_s8 __attribute__((ext_vector_type(8)));
 
@@ -764,13 +768,15 @@ template <int N> __device__ __forceinline__ void pg_load_direct(uint32_t to, con
 constexpr int kPagedTileRows = 128;
 constexpr float paged_tile_lift(bool bf) { return bf ? 0.f : 6.f; }      // of the weight of a score at the reference, log2
 
-template <int D, bool BF>
+template <int D, int CT>
 __global__ __launch_bounds__(256, 2) void paged_tile_kernel(PagedAttnArgs a)
 {
-    constexpr int KS = D / 16, DT = D / 32, CH = D / 8, ROW = 2 * D, STAGE = 2 * 64 * ROW;
+    constexpr bool BF = CT == kPgBf16, BLOCKS = CT == kPgQ8 || CT == kPgQ4;
+    constexpr int KS = D / 16, DT = D / 32, CH = D / 8, ROW = 2 * D, STAGE = 2 * 64 * ROW, KB = D / 32;
     constexpr float kLift = paged_tile_lift(BF), MOST = 32768.f;      // of a lane's weights in a tile: each fits fp16
     typedef typename PgFrag<BF>::type Frag;
     __shared__ __attribute__((aligned(128))) uint8_t lds[2 * STAGE];      // stage: 64 rows of keys, 64 of values
+    __shared__ __attribute__((aligned(16))) uint16_t key_scales[BLOCKS ? 2 * KB * 64 : 1];      // of a stage: [block][key]
     __shared__ uint32_t special;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l32 = lane & 31, hh = lane >> 5;
     const uint32_t head = blockIdx.x % a.c.kv_heads;
@@ -822,9 +828,65 @@ __global__ __launch_bounds__(256, 2) void paged_tile_kernel(PagedAttnArgs a)
         pg_load_direct(to, keys, key_at);
         pg_load_direct(to + 64 * ROW, keys + a.c.half, value_at);
     };
+    // Rows of blocks go through registers: asked for a tile ahead, and stored as fp16 when the tile before is used up.  A unit is 16 codes of 8 bits, or 8 bytes of 4 bits;
+    // keys become integers, whose blocks' sums are scaled in fp32, values are scaled here (2^-11 of each, beside the 16-bit result's own rounding).
+    constexpr int UNITS = D / 16, BLOADS = BLOCKS ? 16 * UNITS / 64 : 1;      // of a row; a lane's
+    typedef typename std::conditional<CT == kPgQ4, pg_u2, pg_u4>::type Unit;
+    Unit ku[BLOADS], vu[BLOADS];
+    uint32_t vs[BLOADS];
+    uint16_t ks[KB];
+    auto fetch = [&](uint32_t page, uint32_t in) {
+        const uint8_t *block = a.c.data + ((uint64_t)(page != kNoPage ? page : 0) * a.c.kv_heads + head) * a.c.block;
+        const uint8_t *keys = block + in * a.c.code_row, *scales = block + (a.c.code_row << a.c.shift) + in * a.c.scale_row;
+#pragma unroll
+        for (int i = 0; i < BLOADS; i++) {
+            const int u = i * 64 + lane;
+            ku[i] = *reinterpret_cast<const Unit *>(keys + (uint32_t)(u * sizeof(Unit)));
+            vu[i] = *reinterpret_cast<const Unit *>(keys + a.c.half + (uint32_t)(u * sizeof(Unit)));
+            vs[i] = *reinterpret_cast<const uint16_t *>(scales + a.c.half + (uint32_t)(u / 2 * 2));
+        }
+#pragma unroll
+        for (int k = 0; k < KB; k++) ks[k] = *reinterpret_cast<const uint16_t *>(scales + (uint32_t)((lane & 15) * (2 * KB) + 2 * k));
+    };
+    auto store = [&](int st, uint32_t kb, bool ok) {
+        uint8_t *kd = lds + st * STAGE + wave * (16 * ROW), *vd = kd + 64 * ROW;
+#pragma unroll
+        for (int i = 0; i < BLOADS; i++) {
+            const int u = i * 64 + lane, row = u / UNITS, in = u % UNITS;
+            const int c0 = CT == kPgQ8 ? 2 * in : in / 2 * 4 + in % 2, c1 = CT == kPgQ8 ? c0 + 1 : c0 + 2;
+            const int kx = row % (CH < 16 ? CH : 16), vx = CH == 8 ? (row / 2 % 2) * 4 : (row % 4) * 4;
+            const uint32_t key = kb + wave * 16 + row;
+            const _Float16 d = __builtin_bit_cast(_Float16, (uint16_t)(key - all.lo < (ok ? all.hi - all.lo : 0u) ? vs[i] : 0u));      // values that no row sees: 0
+            const pg_h2 dd = {d, d};
+            uint32_t w[8];
+            auto unpack = [&](const Unit &x) {
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    if constexpr (CT == kPgQ8) pg_bytes_to_half(x[e] ^ 0x80808080u, 128.f, w[2 * e], w[2 * e + 1]);
+                    else pg_bytes_to_half((e < 2 ? x[e] : x[e - 2] >> 4) & 0x0f0f0f0fu, 8.f, w[2 * e], w[2 * e + 1]);
+                }
+            };
+            unpack(ku[i]);
+            *reinterpret_cast<pg_u4 *>(kd + row * ROW + (c0 ^ kx) * 16) = pg_u4{w[0], w[1], w[2], w[3]};
+            *reinterpret_cast<pg_u4 *>(kd + row * ROW + (c1 ^ kx) * 16) = pg_u4{w[4], w[5], w[6], w[7]};
+            unpack(vu[i]);
+#pragma unroll
+            for (int e = 0; e < 8; e++) w[e] = pg_pk_mul(w[e], dd);
+            *reinterpret_cast<pg_u4 *>(vd + row * ROW + (c0 ^ vx) * 16) = pg_u4{w[0], w[1], w[2], w[3]};
+            *reinterpret_cast<pg_u4 *>(vd + row * ROW + (c1 ^ vx) * 16) = pg_u4{w[4], w[5], w[6], w[7]};
+        }
+        if (lane < 16) {
+#pragma unroll
+            for (int k = 0; k < KB; k++) key_scales[(st * KB + k) * 64 + wave * 16 + lane] = ks[k];
+        }
+    };
     auto page_of = [&](uint32_t at) { return paged_page_uniform(a, table, at); };
-    uint32_t t = s0 * (kPagedStep / 64), mine = kNoPage;
-    if (t < t_end) issue(0, page_of(base + t * 64 + wave * 16), (base + t * 64 + wave * 16) & (psize - 1));
+    uint32_t t = s0 * (kPagedStep / 64), mine = kNoPage, here = kNoPage;
+    if (t < t_end) {
+        here = page_of(base + t * 64 + wave * 16);
+        if constexpr (BLOCKS) fetch(here, (base + t * 64 + wave * 16) & (psize - 1));
+        else issue(0, here, (base + t * 64 + wave * 16) & (psize - 1));
+    }
     if (t + 1 < t_end) mine = page_of(base + (t + 1) * 64 + wave * 16);
 
     // this lane's row
@@ -912,21 +974,40 @@ __global__ __launch_bounds__(256, 2) void paged_tile_kernel(PagedAttnArgs a)
 
     const uint32_t t_first = t;
     int st = 0;
+    if constexpr (BLOCKS) {
+        if (t < t_end) store(0, base + t * 64, here != kNoPage);
+    }
     for (; t < t_end; t++, st ^= 1) {
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        __syncthreads();
+        if constexpr (BLOCKS) {
+            lds_barrier();      // behind it a stage is whole, and the other one, which was read before it, free
+        } else {
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            __syncthreads();
+        }
         auto next = [&]() {
             if (t + 1 >= t_end) return;
-            issue(st ^ 1, mine, (base + (t + 1) * 64 + wave * 16) & (psize - 1));
+            const uint32_t in = (base + (t + 1) * 64 + wave * 16) & (psize - 1);
+            here = mine;
+            if constexpr (BLOCKS) fetch(here, in);
+            else issue(st ^ 1, here, in);
             if (t + 2 < t_end) mine = page_of(base + (t + 2) * 64 + wave * 16);
+        };
+        auto finish = [&]() {
+            if constexpr (BLOCKS) {
+                if (t + 1 < t_end) store(st ^ 1, base + (t + 1) * 64, here != kNoPage);
+            }
         };
         const uint32_t kb = base + t * 64, ok = pages_of(kb);
         uint8_t *kt_lds = lds + st * STAGE, *vt_lds = kt_lds + 64 * ROW;
-        if (partly(kb, ok)) clean(vt_lds, kb, ok);
+        if constexpr (!BLOCKS) {
+            if (partly(kb, ok)) clean(vt_lds, kb, ok);
+        }
         if (idle || kb >= own.hi || kb + 64 <= own.lo) {
             next();
+            finish();
             continue;
         }
+        if constexpr (BLOCKS) next();
         const bool edge = kb < own.all_lo || kb + 64 > own.all_hi || ok != 15;
 
         pg_f16v sc[2];
@@ -934,23 +1015,42 @@ __global__ __launch_bounds__(256, 2) void paged_tile_kernel(PagedAttnArgs a)
         for (int kt = 0; kt < 2; kt++)
 #pragma unroll
             for (int i = 0; i < 16; i++) sc[kt][i] = 0.f;
+        auto key = [&](int kt, int k) {
+            const int row = kt * 32 + l32;
+            return *reinterpret_cast<const Frag *>(kt_lds + row * ROW + ((2 * k + hh) ^ (row % (CH < 16 ? CH : 16))) * 16);
+        };
+        if constexpr (BLOCKS) {
 #pragma unroll
-        for (int k = 0; k < KS; k++)
+            for (int b = 0; b < KB; b++)
 #pragma unroll
-            for (int kt = 0; kt < 2; kt++) {
-                const int row = kt * 32 + l32;
-                const Frag f = *reinterpret_cast<const Frag *>(kt_lds + row * ROW + ((2 * k + hh) ^ (row % (CH < 16 ? CH : 16))) * 16);
-                sc[kt] = pg_mfma32<BF>(f, q[k], sc[kt]);
+                for (int kt = 0; kt < 2; kt++) {
+                    pg_f16v acc;
+#pragma unroll
+                    for (int i = 0; i < 16; i++) acc[i] = 0.f;
+                    acc = pg_mfma32<BF>(key(kt, 2 * b), q[2 * b], acc);
+                    acc = pg_mfma32<BF>(key(kt, 2 * b + 1), q[2 * b + 1], acc);
+#pragma unroll
+                    for (int i = 0; i < 16; i += 4) {
+                        const pg_h4 d = *reinterpret_cast<const pg_h4 *>(key_scales + (st * KB + b) * 64 + 32 * kt + 2 * i + 4 * hh);
+#pragma unroll
+                        for (int e = 0; e < 4; e++) sc[kt][i + e] = fmaf((float)d[e], acc[i + e], sc[kt][i + e]);
+                    }
+                }
+        } else {
+#pragma unroll
+            for (int k = 0; k < KS; k++)
+#pragma unroll
+                for (int kt = 0; kt < 2; kt++) sc[kt] = pg_mfma32<BF>(key(kt, k), q[k], sc[kt]);
+            // reads four products ahead: left alone the compiler reads a pair, waits and multiplies
+            __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
+#pragma unroll
+            for (int k = 0; k < 2 * KS - 4; k++) {
+                __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
             }
-        // reads four products ahead: left alone the compiler reads a pair, waits and multiplies
-        __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
-#pragma unroll
-        for (int k = 0; k < 2 * KS - 4; k++) {
-            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-            __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(0x008, 4, 0);
+            next();      // its scalar work while the products run
         }
-        __builtin_amdgcn_sched_group_barrier(0x008, 4, 0);
-        next();      // its scalar work while the products run
         // score i of kt is key 32 kt + 8 (i / 4) + 4 hh + i % 4
         if (edge) {
             const uint32_t first = kb + 4 * hh - lo;
@@ -998,9 +1098,10 @@ __global__ __launch_bounds__(256, 2) void paged_tile_kernel(PagedAttnArgs a)
         for (int j = 0; j < 4; j++)
 #pragma unroll
             for (int d = 0; d < DT; d++) o[d] = pg_mfma32<BF>(values(vt_lds, d, j), p[j], o[d]);
+        finish();
     }
     __syncthreads();
-    if (special) {
+    if (!BLOCKS && special) {
         // kinds 1 to 3, NaN, inf and -inf: their counts among the keys that a row sees, as a product of ones
         for (t = t_first; t < t_end; t++) {
             const uint32_t kb = base + t * 64, ok = pages_of(kb);

@@ -27,7 +27,7 @@ AttnPlan attn_plan(uint32_t units, uint32_t type, const lv_paged_cache &c, const
     const uint32_t group = s.heads / c.kv_heads;
     const uint64_t mean = (uint64_t)b.tokens * group / b.seqs;      // rows of a sequence and key head
     p.pieces = type == LV_F32 ? (c.type == LV_BF16 ? 3 : 2) : type == LV_F16 && c.type == LV_BF16 ? 3 : 1;
-    const bool tile = p.pieces == 1 && (c.type == LV_F16 || c.type == LV_BF16) && (c.dim == 64 || c.dim == 128) && mean >= kTileRowsMin;
+    const bool tile = p.pieces == 1 && (c.dim == 64 || c.dim == 128) && mean >= kTileRowsMin;
     p.tiles = tile ? 8 : c.dim <= 128 && mean > 16 ? 2 : 1;
     d.seqs = b.seqs;
     d.tokens = b.tokens;
@@ -68,8 +68,12 @@ void launch_attention(const AttnPlan &p, uint32_t grid, hipStream_t st)
     if (p.tiles == 8) {
         lift = paged_tile_lift(bf);
         if constexpr (D == 64 || D == 128) {
-            if (bf) paged_tile_kernel<D, true><<<dim3(grid), dim3(256), 0, st>>>(a);
-            else paged_tile_kernel<D, false><<<dim3(grid), dim3(256), 0, st>>>(a);
+            switch (a.c.type) {
+            case LV_F16: paged_tile_kernel<D, kPgF16><<<dim3(grid), dim3(256), 0, st>>>(a); break;
+            case LV_BF16: paged_tile_kernel<D, kPgBf16><<<dim3(grid), dim3(256), 0, st>>>(a); break;
+            case LV_Q8_0: paged_tile_kernel<D, kPgQ8><<<dim3(grid), dim3(256), 0, st>>>(a); break;
+            default: paged_tile_kernel<D, kPgQ4><<<dim3(grid), dim3(256), 0, st>>>(a); break;
+            }
         }
     } else switch (a.c.type) {
     case LV_F16: p.pieces == 1 ? launch_rows<D, kPgF16, 1>(p, grid, st) : launch_rows<D, kPgF16, 2>(p, grid, st); break;
