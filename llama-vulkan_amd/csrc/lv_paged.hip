@@ -17,7 +17,10 @@ struct AttnPlan {
 
 // Workgroups a compute unit that share the work of a call (lv_paged_plan.h)
 constexpr uint32_t kTargetPerUnit = 2;
-constexpr uint32_t kTileRowsMin = 48;
+// The kernel for tiles takes sequences of more rows than these in the mean (rows of a sequence and key head: new tokens times the heads that share it).  us, rows kernel and
+// tiles, 16 sequences of 3000 keys, 8 key heads of 128: fp16 32 rows 39 40, 40 rows 45 41, 64 rows 47 44, 128 rows 65 51; 8 bits 40 rows 50 52, 64 rows 51 55, 80 rows 79 58
+constexpr uint32_t kTileRows = 32, kTileRowsBlocks = 64;
+// Rows from which the second launch has a wave for each instead of four.
 constexpr uint32_t kJoinRows = 1024;
 
 AttnPlan attn_plan(uint32_t units, uint32_t type, const lv_paged_cache &c, const lv_paged_batch &b, const lv_paged_attn_spec &s)
@@ -27,8 +30,9 @@ AttnPlan attn_plan(uint32_t units, uint32_t type, const lv_paged_cache &c, const
     const uint32_t group = s.heads / c.kv_heads;
     const uint64_t mean = (uint64_t)b.tokens * group / b.seqs;      // rows of a sequence and key head
     p.pieces = type == LV_F32 ? (c.type == LV_BF16 ? 3 : 2) : type == LV_F16 && c.type == LV_BF16 ? 3 : 1;
-    const bool tile = p.pieces == 1 && (c.dim == 64 || c.dim == 128) && mean >= kTileRowsMin;
-    p.tiles = tile ? 8 : c.dim <= 128 && mean > 16 ? 2 : 1;
+    const bool blocks = c.type == LV_Q8_0 || c.type == LV_Q4_0;
+    const bool tile = p.pieces == 1 && (c.dim == 64 || c.dim == 128) && mean > (blocks ? kTileRowsBlocks : kTileRows);
+    p.tiles = tile ? 8 : c.dim <= 128 && mean > 16 ? 2 : 1;      // of 16 rows: keys are read once for each 32 rows where a sequence has more than 16
     d.seqs = b.seqs;
     d.tokens = b.tokens;
     d.group = group;
