@@ -127,6 +127,14 @@ __device__ __forceinline__ uint2 paged_places(const PagedRowsArgs &a, uint32_t r
     return out;
 }
 
+// rint(x * inv) between low and high, 0 for NaN, plus magic
+__device__ __forceinline__ float paged_code(float x, float inv, float low, float high, float magic)
+{
+#pragma clang fp contract(off)
+    const float c = x * inv;
+    return (c == c ? __builtin_amdgcn_fmed3f(c, low, high) : 0.f) + magic;
+}
+
 // eight numbers of a block of 32 as it is stored; the block's are in four neighbouring threads, `quarter` says which
 __device__ __forceinline__ void paged_put_block(const float (&x)[8], bool eight, uint32_t quarter, uint8_t *block_codes, uint16_t *scale)
 {
@@ -147,16 +155,15 @@ __device__ __forceinline__ void paged_put_block(const float (&x)[8], bool eight,
     uint16_t h = float_to_half_bits(s);
     if ((h & 0x7fffu) == 0) h = 0;
     const float back = half_bits_to_float(h), inv = back == 0.f ? 0.f : 1.f / back;
-    const float low = eight ? -127.f : -8.f, high = eight ? 127.f : 7.f;
-    uint32_t lo4 = 0, hi4 = 0;
+    // A number of up to 2^22 plus 1.5 * 2^23 is rounded to an integer, ties to even, whose low byte is the sum's.  The product is rounded first: no fma.
+    const float low = eight ? -127.f : -8.f, high = eight ? 127.f : 7.f, magic = eight ? 12582912.f : 12582920.f;
+    uint32_t b[8];
 #pragma unroll
-    for (int e = 0; e < 8; e++) {
-        const float c = inv == 0.f ? 0.f : fminf(fmaxf(rintf(x[e] * inv), low), high);      // inf times 0 is no number
-        const int q = x[e] == x[e] ? (int)c : 0;
-        const uint32_t bits = (eight ? (uint32_t)q & 0xffu : (uint32_t)(q + 8) & 0xfu) << (8 * (e % 4));
-        if (e < 4) lo4 |= bits;
-        else hi4 |= bits;
-    }
+    for (int e = 0; e < 8; e++) b[e] = __float_as_uint(paged_code(x[e], inv, low, high, magic));
+    auto bytes = [](uint32_t c0, uint32_t c1, uint32_t c2, uint32_t c3) {
+        return __builtin_amdgcn_perm(__builtin_amdgcn_perm(c3, c2, 0x0c0c0400u), __builtin_amdgcn_perm(c1, c0, 0x0c0c0400u), 0x05040100u);
+    };
+    const uint32_t lo4 = bytes(b[0], b[1], b[2], b[3]), hi4 = bytes(b[4], b[5], b[6], b[7]);
     if (quarter == 0) *scale = h;
     if (eight) {
         *reinterpret_cast<uint2 *>(block_codes + quarter * 8) = make_uint2(lo4, hi4);
