@@ -39,6 +39,7 @@ struct PagedAttnArgs {
     uint32_t ldq, ldo, type;
     float scale;                // times log2 e
     const float *sinks;
+    uint32_t items;             // of a key head at most: what `part` has room for
     uint32_t round;             // items of a key head that the device's compute units take at once, or 0
     float *part, *part_ml;      // of cut items: [item][kv head][tile][dim], [item][kv head][tile][2]
 };
@@ -1207,7 +1208,7 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttnArgs a, float 
 #pragma unroll
         for (int j = 0; j < 4; j++) {
             const uint32_t p = p0 + WAVES * j;
-            const uint64_t at = ((uint64_t)(it.first + min(p, it.parts - 1)) * a.c.kv_heads + kvh) * a.deal.tile + in;
+            const uint64_t at = ((uint64_t)min(it.first + min(p, it.parts - 1), a.items - 1) * a.c.kv_heads + kvh) * a.deal.tile + in;
             ms[j] = a.part_ml[2 * at];
             ls[j] = a.part_ml[2 * at + 1];
             if (p >= it.parts) {

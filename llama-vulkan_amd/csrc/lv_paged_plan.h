@@ -93,14 +93,15 @@ LV_HD uint32_t paged_first_key(uint32_t position, uint32_t window, uint32_t chun
 // by token, and some of the keys that they see.  Keys are counted in steps of kPagedStep; a tile that walks `run` steps or up to half as many more is one item, a longer one
 // is cut into equal parts of about so many, whose results a second launch puts together.  The run follows from all lengths at once: the steps of all tiles shared
 // evenly by as many workgroups as the device holds (`target`), so that one long sequence among short ones is cut finely and equal ones are not cut at all
-// when there are enough of them.  us, 2 or 4 or 8 workgroups a compute unit: 131072 keys of one sequence 97, 106, 111; drafts of 16 sequences 23, 27, 28; 64 sequences of 4096 to
+// when there are enough of them.  A workgroup takes `run_min` steps at least.
+// us, 2 or 4 or 8 workgroups a compute unit: 131072 keys of one sequence 97, 106, 111; drafts of 16 sequences 23, 27, 28; 64 sequences of 4096 to
 // 8190 keys 182 when none is cut, 216 with those above the mean cut into a whole run and a rest.
 constexpr uint32_t kPagedStep = 128;
-constexpr uint32_t kPagedRunMin = 2;
 
 struct PagedDeal {
     uint32_t seqs, tokens, group, tile, tile_log2, kv_heads, window, chunk, positions;
     uint32_t target;     // workgroups to share the work; 0: nothing is cut
+    uint32_t run_min;    // steps that a workgroup takes at least
 };
 // steps that a tile of a sequence walks at most: its keys, or as many as a window or a chunk and the tile's tokens cover, and a border on either side
 LV_HD uint32_t paged_steps(const PagedDeal &d, const PagedSeq &s)
@@ -118,7 +119,7 @@ LV_HD uint32_t paged_run(const PagedDeal &d, float all_steps)
 {
     if (!d.target) return 0x7fffffffu;
     const float run = all_steps * (float)d.kv_heads / (float)d.target;
-    return run < (float)kPagedRunMin ? kPagedRunMin : run > 1e9f ? 1000000000u : (uint32_t)run + 1;
+    return run < (float)d.run_min ? d.run_min : run > 1e9f ? 1000000000u : (uint32_t)run + 1;
 }
 LV_HD uint32_t paged_parts(uint32_t steps, uint32_t run)
 {

@@ -292,6 +292,19 @@ def test_attention_of_one_long_sequence(dev, cache, kind):
     check_attention(dev, np.random.default_rng(36), cache, kind, 4, 1, 64, 64, [6001, 3], [2, 1], sinks=True)
 
 
+@pytest.mark.parametrize("cache,kind", TYPES, ids=lambda k: ref.NAMES[k])
+@pytest.mark.parametrize("dim", [32, 64, 128, 256])
+def test_attention_cut_and_whole_in_one_call(dev, cache, kind, dim):
+    """a table of more than 384 positions: sequences of several steps are cut, those beside them are not"""
+    check_attention(dev, np.random.default_rng(50), cache, kind, 4, 2, dim, 16, [1, 130, 450, 33], [1, 1, 1, 0], pad=1, sinks=True)
+    check_attention(dev, np.random.default_rng(51), cache, kind, 3, 1, dim, 32, [40, 500, 7], [40, 30, 3], pad=2)
+
+
+def test_attention_of_chunks_that_are_not_cut(dev):
+    """more than 384 positions and workgroups for half of the compute units: one launch, of a table that leaves nothing to cut"""
+    check_attention(dev, np.random.default_rng(52), F16, F16, 32, 32, 64, 64, [700], [700])
+
+
 def test_attention_of_many_sequences(dev):
     rng = np.random.default_rng(37)
     lens = rng.integers(1, 60, 150)
@@ -438,10 +451,12 @@ def test_attention_of_a_pool_beyond_32_bits(dev):
 def test_attention_workspace_refusals(dev):
     lva, ctx = dev.lva, dev.ctx
     rng = np.random.default_rng(43)
-    pool = ref.Pool(F16, 1, 64, 16, 8, rng)
+    pool = ref.Pool(F16, 1, 64, 16, 40, rng)
     step = ref.Step(pool, [100], [1], rng)
     _, c = dev.cache(pool)
     b, spec = dev.batch(step), lva.PagedAttnSpec(2, 0.1, 0, 0, None)
+    assert ctx.paged_attention_workspace(F16, c, b, spec) == 0      # a table of so few positions is not cut
+    b = dev.batch(ref.Step(pool, [500], [1], rng))
     n = ctx.paged_attention_workspace(F16, c, b, spec)
     assert n > 0
     p = dev.put(np.zeros((2, 128), np.float16))

@@ -198,7 +198,7 @@ int main()
             printf("%u\n", lv::paged_first_key(p, w, c));
         } else if (what == "deal") {
             lv::PagedDeal d{};
-            std::cin >> d.seqs >> d.group >> d.tile >> d.kv_heads >> d.window >> d.chunk >> d.positions >> d.target;
+            std::cin >> d.seqs >> d.group >> d.tile >> d.kv_heads >> d.window >> d.chunk >> d.positions >> d.target >> d.run_min;
             while (1u << d.tile_log2 < d.tile) d.tile_log2++;
             std::vector<uint32_t> lens(d.seqs), news(d.seqs);
             for (uint32_t b = 0; b < d.seqs; b++) std::cin >> lens[b] >> news[b], d.tokens += news[b];
@@ -301,7 +301,7 @@ def test_every_key_is_dealt(ask):
         if n % 5 == 0:
             lens[0] = 200000
         qs.append(("deal", seqs, int(rng.integers(1, 9)), int(rng.choice([16, 32, 64, 128])), int(rng.choice([1, 4, 8, 40])), int(rng.choice([0, 0, 7, 512])),
-                   int(rng.choice([0, 0, 10, 1000])), 1 << 20, int(rng.choice([0, 256, 1024])), *np.stack([lens, new], 1).reshape(-1).tolist()))
+                   int(rng.choice([0, 0, 10, 1000])), 1 << 20, int(rng.choice([0, 256, 1024])), int(rng.choice([1, 1, 9])), *np.stack([lens, new], 1).reshape(-1).tolist()))
     cut = 0
     for q, (run, items, room, missed, c) in zip(qs, ask(qs)):
         assert missed == 0 and items <= room, q[:9]
@@ -311,9 +311,11 @@ def test_every_key_is_dealt(ask):
 
 
 def test_one_long_sequence_is_cut_and_equal_ones_are_not(ask):
-    one = ask([("deal", 1, 4, 16, 8, 0, 0, 1 << 20, 1024, 131072, 1)])[0]
+    one = ask([("deal", 1, 4, 16, 8, 0, 0, 1 << 20, 1024, 1, 131072, 1)])[0]
     assert one[1] >= 100 and one[4] == 1
-    many = ask([("deal", 128, 4, 16, 8, 0, 0, 1 << 20, 1024, *([4096, 1] * 128))])[0]
+    many = ask([("deal", 128, 4, 16, 8, 0, 0, 1 << 20, 1024, 1, *([4096, 1] * 128))])[0]
     assert many[1] <= 2 * 128
-    mixed = ask([("deal", 64, 4, 16, 8, 0, 0, 1 << 20, 1024, 131072, 1, *([100, 1] * 63))])[0]
+    mixed = ask([("deal", 64, 4, 16, 8, 0, 0, 1 << 20, 1024, 1, 131072, 1, *([100, 1] * 63))])[0]
     assert mixed[1] >= 100 + 63 and mixed[4] == 1
+    short = ("deal", 4, 4, 128, 8, 0, 0, 1 << 20, 1024)
+    assert ask([(*short, 1, *([1000, 300] * 4))])[0][4] == 4 and ask([(*short, 9, *([1000, 300] * 4))])[0][4] == 0
