@@ -279,12 +279,16 @@ __device__ __forceinline__ pg_s4 pg_read_columns(const uint8_t *p)
 
 // ---- rows: single tokens, drafts, 32-bit queries -----------------------------------------------------------------------------------
 // A workgroup's tile is 16 QT rows; its four waves take turns of 32 keys and never wait for one another before the end, where their results are put
-// together.  Keys go from memory to registers as the first operand, values through the wave's own 32 rows of LDS; the next turn's are asked
-// for before this turn's are used.  Bound by the bytes of the cache.
+// together.  Keys of 16 bits go from memory to registers as the first operand, values, and codes and scales of both, through the wave's own 32 rows of LDS; the next
+// turn's are asked for before this turn's are used.  Bound by the bytes of the cache where there are many (131072 keys of 8 heads in fp16 99 us, 5.4 TB/s; 64 sequences of 8 bits
+// 174 us, 4.9 TB/s); with few keys by a chain of loads, each about 2000 clocks: lengths, the first pages, the first keys.
 //
 // NQ: pieces of a query, 1, or with 32-bit queries 2 (fp16 rows: 22 bits) or 3 (bf16 rows: 24 bits); the weights have as many, 2 of bf16 at least.  Rows of
 // codes: keys enter as exact integers, a block's sum is scaled in fp32.  Values are scaled in fp16 (a rounding of 2^-11 of each, beside the 16-bit result's own); with
 // 32-bit queries they enter as two fp16 pieces, which hold them exactly: 19 bits at most, the last of them 2^-24 or more, as the scale's is.
+typedef uint32_t pg_u2 __attribute__((ext_vector_type(2)));
+template <int BYTES> struct PgWord { typedef uint32_t type; };
+template <> struct PgWord<8> { typedef pg_u2 type; };
 // waves a SIMD that the registers are cut for: as many as leave none in memory
 constexpr int paged_rows_waves(int D, int CT, int NQ, int QT)
 {
@@ -299,7 +303,7 @@ __global__ __launch_bounds__(256, paged_rows_waves(D, CT, NQ, QT)) void paged_ro
 {
     constexpr bool BF = CT == kPgBf16, BLOCKS = CT == kPgQ8 || CT == kPgQ4, EXACT = NQ > 1;
     constexpr int KS = D / 32, DT = D / 16, CH = D / 8, ROW = 2 * D + 16, NP = BF && NQ == 1 ? 2 : NQ, TILE = 16 * QT;
-    constexpr float kLift = BF ? 0.f : 12.f;
+    constexpr float kLift = BF ? 0.f : 12.f, kRoom = 3.f;
     constexpr int MERGE = D + 4;                      // floats of a row of results in LDS
     typedef typename PgFrag<BF>::type Frag;
     constexpr int PLANES = BLOCKS && EXACT ? 2 : 1, VALUES = 32 * ROW * PLANES;      // bytes of a wave's 32 rows of values; 16 more a row put the 16 rows of a column read on all banks evenly
@@ -342,20 +346,18 @@ __global__ __launch_bounds__(256, paged_rows_waves(D, CT, NQ, QT)) void paged_ro
     const uint32_t turns = n_steps ? (k_hi - base + 31) / 32 : 0, t_end = min(s1 * 4, turns);
     uint8_t *mine = lds + wave * VALUES;
 
+    // row of 32 and unit of 16 bytes of the row that this lane brings with its i-th load of values, and of keys that are codes
+    constexpr int UNITS = BLOCKS ? (CT == kPgQ8 ? D : D / 2) / 16 : CH, LOADS = UNITS > 1 ? 32 * UNITS / 64 : 1;
+    // the scales of 32 rows are asked for as words in one load
+    constexpr int WORD = D == 256 ? 8 : 4, WORDS = 2 * D / WORD;
+    typedef typename PgWord<WORD>::type Word;
     struct Turn {
-        uint4 k4[CT <= kPgBf16 ? 2 : 1][CT <= kPgBf16 ? KS : 1];
-        uint2 k2[CT == kPgQ8 ? 2 : 1][CT == kPgQ8 ? KS : 1];
-        uint32_t k1[CT == kPgQ4 ? 2 : 1][CT == kPgQ4 ? KS : 1];
-        uint2 ks[BLOCKS ? 2 : 1][BLOCKS ? KS : 1];                          // scales of keys 4 g .. 4 g + 3 of 16: [key][block]
-        uint4 v4[CT <= kPgBf16 ? D / 16 : CT == kPgQ8 ? D / 32 : 1];        // 16 bytes of a row
-        uint2 v2[CT == kPgQ4 ? D / 32 : 1];                                 // 8 bytes: half a block's
-        uint16_t vd[BLOCKS ? D / 32 : 1];
+        pg_u4 k4[BLOCKS ? 1 : 2][BLOCKS ? LOADS : KS], v4[LOADS];
+        Word ks, vs;
     };
-    // row of 32 and unit of the row that this lane brings with its i-th load of values
-    constexpr int UNITS = CT <= kPgBf16 ? CH : D / 16, LOADS = 32 * UNITS / 64;
     // (addresses are made anew in every turn, from a lane number that the compiler cannot see through: kept, they would take a hundred registers)
     int ln = lane;
-    auto row_of = [&](int i) { return (i * 64 + ln) / UNITS; };
+    auto row_of = [&](int i) { return UNITS > 1 ? (i * 64 + ln) / UNITS : ln % 32; };
     auto unit_of = [&](int i) { return (i * 64 + ln) % UNITS; };
     // where 16 keys' codes lie (of keys; of values and scales at the same distances in every block), null without a page
     Turn x;
@@ -367,34 +369,66 @@ __global__ __launch_bounds__(256, paged_rows_waves(D, CT, NQ, QT)) void paged_ro
     auto block_of = [&](uint32_t page) { return a.c.data + ((uint64_t)(page != kNoPage ? page : 0) * a.c.kv_heads + head) * a.c.block; };
     const uint32_t scales_at = a.c.code_row << a.c.shift;
     auto load_keys = [&](uint32_t page0, uint32_t page1, uint32_t in0, uint32_t in1) {
+        if constexpr (BLOCKS) {
+            const uint8_t *block0 = block_of(page0), *block1 = block_of(page1);
+            const uint8_t *pk0 = block0 + in0 * a.c.code_row, *pk1 = block1 + in1 * a.c.code_row;
 #pragma unroll
-        for (int kt = 0; kt < 2; kt++) {
-            const uint8_t *block = block_of(kt ? page1 : page0);
-            const uint32_t in = kt ? in1 : in0;
-            const uint8_t *pk = block + in * a.c.code_row, *ps = block + scales_at + in * a.c.scale_row;
+            for (int i = 0; i < LOADS; i++) {
+                const int row = row_of(i), u = unit_of(i);
+                const bool second = 64 / UNITS <= 16 ? i * (64 / UNITS) >= 16 : row >= 16;
+                x.k4[0][i] = *reinterpret_cast<const pg_u4 *>((second ? pk1 : pk0) + (uint32_t)((row & 15) * (UNITS * 16) + u * 16));
+            }
+            const uint32_t at = (uint32_t)(ln % WORDS) * WORD;
+            const uint8_t *ps = (at < D ? block0 + in0 * a.c.scale_row : block1 + in1 * a.c.scale_row) + scales_at + at % D;
+            x.ks = *reinterpret_cast<const Word *>(ps);
+            x.vs = *reinterpret_cast<const Word *>(ps + a.c.half);
+        } else {
 #pragma unroll
-            for (int k = 0; k < KS; k++) {
-                if constexpr (CT <= kPgBf16) x.k4[kt][k] = *reinterpret_cast<const uint4 *>(pk + (uint32_t)((ln & 15) * (2 * D) + k * 64 + (ln >> 4) * 16));
-                else if constexpr (CT == kPgQ8) x.k2[kt][k] = *reinterpret_cast<const uint2 *>(pk + (uint32_t)((ln & 15) * D + k * 32 + (ln >> 4) * 8));
-                else x.k1[kt][k] = *reinterpret_cast<const uint32_t *>(pk + (uint32_t)((ln & 15) * (D / 2) + k * 16 + (ln >> 4) * 4));
-                if constexpr (BLOCKS) x.ks[kt][k] = *reinterpret_cast<const uint2 *>(ps + (uint32_t)((ln >> 4) * (D / 4) + k * 8));
+            for (int kt = 0; kt < 2; kt++) {
+                const uint8_t *pk = block_of(kt ? page1 : page0) + (kt ? in1 : in0) * a.c.code_row;
+#pragma unroll
+                for (int k = 0; k < KS; k++) x.k4[kt][k] = *reinterpret_cast<const pg_u4 *>(pk + (uint32_t)((ln & 15) * (2 * D) + k * 64 + (ln >> 4) * 16));
             }
         }
     };
     auto load_values = [&](uint32_t page0, uint32_t page1, uint32_t in0, uint32_t in1) {
-        const uint8_t *block0 = block_of(page0) + a.c.half, *block1 = block_of(page1) + a.c.half;
-        const uint8_t *pv0 = block0 + in0 * a.c.code_row, *pv1 = block1 + in1 * a.c.code_row;
-        const uint8_t *ps0 = block0 + scales_at + in0 * a.c.scale_row, *ps1 = block1 + scales_at + in1 * a.c.scale_row;
+        const uint8_t *pv0 = block_of(page0) + a.c.half + in0 * a.c.code_row, *pv1 = block_of(page1) + a.c.half + in1 * a.c.code_row;
 #pragma unroll
         for (int i = 0; i < LOADS; i++) {
             const int row = row_of(i), u = unit_of(i);
             const bool second = 64 / UNITS <= 16 ? i * (64 / UNITS) >= 16 : row >= 16;      // of 16 keys; where a load covers no more, the same in all lanes
-            const uint8_t *p = second ? pv1 : pv0, *ps = second ? ps1 : ps0;
-            if constexpr (CT <= kPgBf16) x.v4[i] = *reinterpret_cast<const uint4 *>(p + (uint32_t)((row & 15) * (2 * D) + u * 16));
-            else if constexpr (CT == kPgQ8) x.v4[i] = *reinterpret_cast<const uint4 *>(p + (uint32_t)((row & 15) * D + u * 16));
-            else x.v2[i] = *reinterpret_cast<const uint2 *>(p + (uint32_t)((row & 15) * (D / 2) + u * 8));
-            if constexpr (BLOCKS) x.vd[i] = *reinterpret_cast<const uint16_t *>(ps + (uint32_t)((row & 15) * (D / 16) + u / 2 * 2));
+            x.v4[i] = *reinterpret_cast<const pg_u4 *>((second ? pv1 : pv0) + (uint32_t)((row & 15) * (UNITS * 16) + u * 16));
         }
+    };
+    // Codes of keys, and scales, pass through the place of the values, which is free then: loads of 16 bytes in a row and one for 32 rows' scales, where each lane's own
+    // 4 or 8 bytes of a row would take three times the loads and four times the caches' accesses.  Units of a row change places by its number, so that 64 lanes read all banks.
+    constexpr int KSC = 32 * UNITS * 16, VSC = KSC + 2 * D;
+    auto unit_at = [&](int row, int u) { return row * (UNITS * 16) + (u ^ (row * UNITS / 16 & (UNITS - 1))) * 16; };
+    pg_u2 kw[BLOCKS ? 2 : 1][BLOCKS ? KS : 1];      // codes of key (lane & 15)
+    pg_u2 ks[BLOCKS ? 2 : 1][BLOCKS ? KS : 1];                              // scales of keys 4 g .. 4 g + 3 of 16: [key][block]
+    uint16_t vd[BLOCKS ? LOADS : 1];
+    auto turn_keys = [&]() {
+#pragma unroll
+        for (int i = 0; i < LOADS; i++) *reinterpret_cast<pg_u4 *>(mine + unit_at(row_of(i), unit_of(i))) = x.k4[0][i];
+        const int at = ln % WORDS * WORD;
+        *reinterpret_cast<Word *>(mine + KSC + at) = x.ks;
+        *reinterpret_cast<Word *>(mine + VSC + at) = x.vs;
+    };
+    auto take_keys = [&]() {
+#pragma unroll
+        for (int kt = 0; kt < 2; kt++)
+#pragma unroll
+            for (int k = 0; k < KS; k++) {
+                const int row = kt * 16 + (ln & 15), g = ln >> 4;
+                if constexpr (CT == kPgQ8) {
+                    kw[kt][k] = *reinterpret_cast<const pg_u2 *>(mine + unit_at(row, 2 * k + g / 2) + g % 2 * 8);
+                } else {
+                    kw[kt][k].x = *reinterpret_cast<const uint32_t *>(mine + unit_at(row, k) + g * 4);
+                }
+                ks[kt][k] = *reinterpret_cast<const pg_u2 *>(mine + KSC + (kt * 16 + g * 4) * (D / 16) + k * 8);
+            }
+#pragma unroll
+        for (int i = 0; i < LOADS; i++) vd[i] = *reinterpret_cast<const uint16_t *>(mine + VSC + row_of(i) * (D / 16) + (CT == kPgQ8 ? unit_of(i) / 2 : unit_of(i)) * 2);
     };
 
     pg_f4 o[DT][QT];
@@ -424,9 +458,9 @@ __global__ __launch_bounds__(256, paged_rows_waves(D, CT, NQ, QT)) void paged_ro
             const int row = row_of(i);
             const bool keep = kb + row - k_lo < ((row < 16 ? ok0 : ok1) ? k_hi - k_lo : 0u);
             if constexpr (CT <= kPgBf16) {
-                if (!keep) x.v4[i] = make_uint4(0, 0, 0, 0);
+                if (!keep) x.v4[i] = pg_u4{0, 0, 0, 0};
             } else {
-                if (!keep) x.vd[i] = 0;
+                if (!keep) vd[i] = 0;
             }
         }
     };
@@ -440,13 +474,18 @@ __global__ __launch_bounds__(256, paged_rows_waves(D, CT, NQ, QT)) void paged_ro
     };
     bool special = false;
     const uint32_t t_first = s0 * 4 + wave;
-    uint32_t t = t_first, page0 = kNoPage, page1 = kNoPage;
+    uint32_t t = t_first, page0 = kNoPage, page1 = kNoPage, in0 = 0, in1 = 0, next0 = kNoPage, next1 = kNoPage;
     if (t < t_end) {
-        uint32_t in0, in1;
         page0 = place(t, 0, in0);
         page1 = place(t, 1, in1);
         load_keys(page0, page1, in0, in1);
         load_values(page0, page1, in0, in1);
+        // (the last turn asks for its own again, which are in the caches: a condition around the loads costs registers)
+        if constexpr (BLOCKS) {
+            const uint32_t next = t + 4 < t_end ? t + 4 : t;
+            next0 = place(next, 0, in0);
+            next1 = place(next, 1, in1);
+        }
     }
 
     Frag q[QT][KS][NQ];
@@ -487,12 +526,28 @@ __global__ __launch_bounds__(256, paged_rows_waves(D, CT, NQ, QT)) void paged_ro
         const bool ok0 = page0 != kNoPage, ok1 = page1 != kNoPage;
         const bool inside = kb >= k_lo && kb + 32 <= k_hi && ok0 && ok1;                // every key of the turn is some row's
         const bool edge = kb < all_lo || kb + 32 > all_hi || !inside;                   // some row does not see all of them
-        // the next turn's pages; its keys are asked for as soon as this turn's are used up, its values likewise
-        // (the last one asks for its own again, which are in the caches: a condition around the loads costs registers)
+        // The next turn's keys are asked for as soon as this turn's are used up, its values likewise; their pages are known from the turn before
         const uint32_t next = t + 4 < t_end ? t + 4 : t;
-        uint32_t in0, in1;
-        page0 = place(next, 0, in0);
-        page1 = place(next, 1, in1);
+        if constexpr (!BLOCKS) {
+            next0 = place(next, 0, in0);
+            next1 = place(next, 1, in1);
+        }
+        page0 = next0;
+        page1 = next1;
+        const uint32_t at0 = in0, at1 = in1;
+        if constexpr (BLOCKS) {
+            turn_keys();
+            __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+            __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+            load_keys(page0, page1, at0, at1);
+            take_keys();
+        }
+        if constexpr (BLOCKS) {
+            const uint32_t then = next + 4 < t_end ? next + 4 : next;
+            next0 = place(then, 0, in0);
+            next1 = place(then, 1, in1);
+        }
         pg_f4 sc[2][QT];
 #pragma unroll
         for (int kt = 0; kt < 2; kt++) {
@@ -506,11 +561,11 @@ __global__ __launch_bounds__(256, paged_rows_waves(D, CT, NQ, QT)) void paged_ro
                 } else {
                     uint4 w;
                     if constexpr (CT == kPgQ8) {
-                        pg_bytes_to_half(x.k2[kt][k].x ^ 0x80808080u, 128.f, w.x, w.y);
-                        pg_bytes_to_half(x.k2[kt][k].y ^ 0x80808080u, 128.f, w.z, w.w);
+                        pg_bytes_to_half(kw[kt][k].x ^ 0x80808080u, 128.f, w.x, w.y);
+                        pg_bytes_to_half(kw[kt][k].y ^ 0x80808080u, 128.f, w.z, w.w);
                     } else {
-                        pg_bytes_to_half(x.k1[kt][k] & 0x0f0f0f0fu, 8.f, w.x, w.y);
-                        pg_bytes_to_half((x.k1[kt][k] >> 4) & 0x0f0f0f0fu, 8.f, w.z, w.w);
+                        pg_bytes_to_half(kw[kt][k].x & 0x0f0f0f0fu, 8.f, w.x, w.y);
+                        pg_bytes_to_half((kw[kt][k].x >> 4) & 0x0f0f0f0fu, 8.f, w.z, w.w);
                     }
                     f = __builtin_bit_cast(Frag, w);
                 }
@@ -523,7 +578,7 @@ __global__ __launch_bounds__(256, paged_rows_waves(D, CT, NQ, QT)) void paged_ro
 #pragma unroll
                         for (int r = 0; r < 4; r++) {
                             const int at = r * KS + k;      // half at / of ks: [key][block]
-                            const uint32_t word = at % 4 < 2 ? x.ks[kt][at / 4].x : x.ks[kt][at / 4].y;
+                            const uint32_t word = at % 4 < 2 ? ks[kt][at / 4].x : ks[kt][at / 4].y;
                             sc[kt][i][r] = fmaf(half_bits_to_float((uint16_t)(word >> (at % 2 * 16))), acc[r], sc[kt][i][r]);
                         }
                     } else {
@@ -532,7 +587,7 @@ __global__ __launch_bounds__(256, paged_rows_waves(D, CT, NQ, QT)) void paged_ro
                 }
             }
         }
-        load_keys(page0, page1, in0, in1);
+        if constexpr (!BLOCKS) load_keys(page0, page1, at0, at1);
         Frag p[QT][NP];
 #pragma unroll
         for (int i = 0; i < QT; i++) {
@@ -547,7 +602,8 @@ __global__ __launch_bounds__(256, paged_rows_waves(D, CT, NQ, QT)) void paged_ro
             for (int e = 0; e < 8; e++) top = fmaxf(top, s[e]);
             top = fmaxf(top, __shfl_xor(top, 16, 64));
             top = fmaxf(top, __shfl_xor(top, 32, 64));
-            if (__any(top > m[i])) {
+            // the reference follows the maximum where it is more than kRoom behind: weights stay below 2^15, and most turns leave the results as they are
+            if (__any(top > m[i] + kRoom)) {
                 const float f = pg_exp2(m[i] - top);
                 m[i] = top;
                 l[i] *= f;
@@ -571,47 +627,44 @@ __global__ __launch_bounds__(256, paged_rows_waves(D, CT, NQ, QT)) void paged_ro
         if (CT <= kPgBf16 && any_special()) {
             special = true;
 #pragma unroll
-            for (int i = 0; i < (CT <= kPgBf16 ? LOADS : 0); i++) x.v4[i] = __builtin_bit_cast(uint4, pg_only<BF>(__builtin_bit_cast(Frag, x.v4[i]), 0));
+            for (int i = 0; i < (CT <= kPgBf16 ? LOADS : 0); i++) x.v4[i] = __builtin_bit_cast(pg_u4, pg_only<BF>(__builtin_bit_cast(Frag, x.v4[i]), 0));
         }
 #pragma unroll
         for (int i = 0; i < LOADS; i++) {
             const int row = row_of(i), u = unit_of(i);
             if constexpr (CT <= kPgBf16) {
-                put(row, u, x.v4[i]);
+                put(row, u, __builtin_bit_cast(uint4, x.v4[i]));
             } else {
-                uint4 w0, w1;
-                if constexpr (CT == kPgQ8) {
-                    pg_bytes_to_half(x.v4[i].x ^ 0x80808080u, 128.f, w0.x, w0.y);
-                    pg_bytes_to_half(x.v4[i].y ^ 0x80808080u, 128.f, w0.z, w0.w);
-                    pg_bytes_to_half(x.v4[i].z ^ 0x80808080u, 128.f, w1.x, w1.y);
-                    pg_bytes_to_half(x.v4[i].w ^ 0x80808080u, 128.f, w1.z, w1.w);
-                } else {
-                    pg_bytes_to_half(x.v2[i].x & 0x0f0f0f0fu, 8.f, w0.x, w0.y);
-                    pg_bytes_to_half(x.v2[i].y & 0x0f0f0f0fu, 8.f, w0.z, w0.w);
-                    pg_bytes_to_half((x.v2[i].x >> 4) & 0x0f0f0f0fu, 8.f, w1.x, w1.y);
-                    pg_bytes_to_half((x.v2[i].y >> 4) & 0x0f0f0f0fu, 8.f, w1.z, w1.w);
-                }
-                const _Float16 d = __builtin_bit_cast(_Float16, x.vd[i]);
-                const int c0 = CT == kPgQ8 ? 2 * u : u / 2 * 4 + u % 2, c1 = CT == kPgQ8 ? c0 + 1 : c0 + 2;
-                if constexpr (EXACT) {
-                    auto cut = [&](uint4 w, int ch) {
+                const pg_u4 c = x.v4[i];
+                const _Float16 d = __builtin_bit_cast(_Float16, vd[i]);
+                auto values_of = [&](uint32_t c0, uint32_t c1, float bias, int ch) {      // eight bytes' numbers into a chunk
+                    uint4 w;
+                    pg_bytes_to_half(c0, bias, w.x, w.y);
+                    pg_bytes_to_half(c1, bias, w.z, w.w);
+                    if constexpr (EXACT) {
                         const pg_h8 code = __builtin_bit_cast(pg_h8, w);
                         pg_h8 piece[2];
 #pragma unroll
                         for (int e = 0; e < 8; e++) pg_cut<false, 2>((float)code[e] * (float)d, e, piece);
                         put(row, ch, __builtin_bit_cast(uint4, piece[0]));
                         put(row, ch, __builtin_bit_cast(uint4, piece[1]), 1);
-                    };
-                    cut(w0, c0);
-                    cut(w1, c1);
-                } else {
-                    const pg_h2 dd = {d, d};
-                    put(row, c0, make_uint4(pg_pk_mul(w0.x, dd), pg_pk_mul(w0.y, dd), pg_pk_mul(w0.z, dd), pg_pk_mul(w0.w, dd)));
-                    put(row, c1, make_uint4(pg_pk_mul(w1.x, dd), pg_pk_mul(w1.y, dd), pg_pk_mul(w1.z, dd), pg_pk_mul(w1.w, dd)));
+                    } else {
+                        const pg_h2 dd = {d, d};
+                        put(row, ch, make_uint4(pg_pk_mul(w.x, dd), pg_pk_mul(w.y, dd), pg_pk_mul(w.z, dd), pg_pk_mul(w.w, dd)));
+                    }
+                };
+#pragma unroll
+                for (int j = 0; j < 2; j++) {
+                    if constexpr (CT == kPgQ8) {
+                        values_of(c[2 * j] ^ 0x80808080u, c[2 * j + 1] ^ 0x80808080u, 128.f, 2 * u + j);
+                    } else {
+                        values_of(c[2 * j] & 0x0f0f0f0fu, c[2 * j + 1] & 0x0f0f0f0fu, 8.f, 4 * u + j);
+                        values_of((c[2 * j] >> 4) & 0x0f0f0f0fu, (c[2 * j + 1] >> 4) & 0x0f0f0f0fu, 8.f, 4 * u + 2 + j);
+                    }
                 }
             }
         }
-        load_values(page0, page1, in0, in1);
+        load_values(page0, page1, at0, at1);
 #pragma unroll
         for (int d = 0; d < DT; d++) {
             if constexpr (PLANES == 2) {      // the smaller pieces first; the product of both smaller ones is 2^-22 of the whole
@@ -630,7 +683,6 @@ __global__ __launch_bounds__(256, paged_rows_waves(D, CT, NQ, QT)) void paged_ro
     if (CT <= kPgBf16 && special) {
         for (t = t_first; t < t_end; t += 4) {
             const uint32_t kb = base + t * 32;
-            uint32_t in0, in1;
             page0 = place(t, 0, in0);
             page1 = place(t, 1, in1);
             const bool ok0 = page0 != kNoPage, ok1 = page1 != kNoPage;
@@ -638,7 +690,7 @@ __global__ __launch_bounds__(256, paged_rows_waves(D, CT, NQ, QT)) void paged_ro
             clear(kb, ok0, ok1);
             if (!any_special()) continue;
 #pragma unroll
-            for (int i = 0; i < (CT <= kPgBf16 ? LOADS : 0); i++) put(row_of(i), unit_of(i), x.v4[i]);
+            for (int i = 0; i < (CT <= kPgBf16 ? LOADS : 0); i++) put(row_of(i), unit_of(i), __builtin_bit_cast(uint4, x.v4[i]));
             // 1: NaN, 2: inf, 3: -inf.  Counts of each among the keys that a row sees, as a product of ones
 #pragma unroll 1
             for (int kind = 1; kind <= 3; kind++) {

@@ -28,6 +28,10 @@ constexpr uint32_t kWholeKeys = 384;
 // ... and chunks, where half of the compute units have a workgroup, whose tiles walk fewer than one and a half times these steps (us, steps of 2 and of 9 at least, fp16: 512
 // tokens over 32 key heads 33 20, 1024 over 8 44 29, 1000 behind 500 52 41; 512 behind 1536 42 42, and 53 with steps of 12).
 constexpr uint32_t kTileRun = 9;
+// Where every compute unit has a workgroup without a cut, sequences are cut for evenness only: into more workgroups than are there at once, which follow as others end, and
+// of many steps.  us, 2 a unit of one step at least, 6 of 8, 6 of 16: 64 sequences of 4096 .. 8190 keys, 8 heads of 8 bits 184 174 174; 128 of 1000 .. 2000 of 8 heads in fp16
+// 147 153 143; 32 of 2000 .. 4000 84 80 89; 16 of 1000 .. 2000 of 32 heads 80 83 77; 8 of 511 of 32 heads 19.5 15.4 15.4.
+constexpr uint32_t kManyPerUnit = 6, kManyRun = 8, kManyMoreRun = 16;
 
 AttnPlan attn_plan(uint32_t units, uint32_t type, const lv_paged_cache &c, const lv_paged_batch &b, const lv_paged_attn_spec &s)
 {
@@ -50,7 +54,12 @@ AttnPlan attn_plan(uint32_t units, uint32_t type, const lv_paged_cache &c, const
     d.positions = b.table_ld * c.page;
     d.target = kTargetPerUnit * units;
     const uint64_t whole = (uint64_t)b.tokens * group / d.tile * c.kv_heads;      // workgroups if nothing is cut
+    const uint64_t least = (uint64_t)std::min(b.seqs, b.tokens) * c.kv_heads;     // sequences' key heads with something to do, if all have
     d.run_min = tile && whole >= units / 2 ? kTileRun : 1;
+    if (!tile && least >= units) {
+        d.target = kManyPerUnit * units;
+        d.run_min = least >= 2 * units ? kManyMoreRun : kManyRun;
+    }
     PagedSeq longest{};
     longest.keys = d.positions;
     if (whole >= d.target || d.positions <= kWholeKeys || paged_parts(paged_steps(d, longest), d.run_min) == 1) d.target = 0;

@@ -94,8 +94,7 @@ LV_HD uint32_t paged_first_key(uint32_t position, uint32_t window, uint32_t chun
 // is cut into equal parts of about so many, whose results a second launch puts together.  The run follows from all lengths at once: the steps of all tiles shared
 // evenly by as many workgroups as the device holds (`target`), so that one long sequence among short ones is cut finely and equal ones are not cut at all
 // when there are enough of them.  A workgroup takes `run_min` steps at least.
-// us, 2 or 4 or 8 workgroups a compute unit: 131072 keys of one sequence 97, 106, 111; drafts of 16 sequences 23, 27, 28; 64 sequences of 4096 to
-// 8190 keys 182 when none is cut, 216 with those above the mean cut into a whole run and a rest.
+// us, 2 or 4 or 8 workgroups a compute unit: 131072 keys of one sequence 99, 106, 111; drafts of 16 sequences 20.4, 21.3, 21.4.
 constexpr uint32_t kPagedStep = 128;
 
 struct PagedDeal {
