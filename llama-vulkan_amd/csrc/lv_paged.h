@@ -6,7 +6,7 @@
 // from row-major values through ds_read_b64_tr_b16, which hands lane i of 16 the column i of 4 rows.
 //
 // Scores are in units of log2, 2^12 on top of the weights of fp16 products (a weight below 2^-14 of the largest would be an fp16 subnormal), which the sum has
-// as well.  Masked scores are -inf, the running maximum starts at a finite -1e30: a row that sees nothing ends with a sum of 0 and is written as 0.
+// as well.  Masked scores are -inf, the running maximum starts at kNothing, finite and below all scores: a row that sees nothing ends with a sum of 0 and is written as 0.
 #pragma once
 
 #include <type_traits>
@@ -53,6 +53,8 @@ __device__ __forceinline__ uint32_t paged_page_uniform(const PagedAttnArgs &a, c
     if (i < a.table_ld) p = *((const __attribute__((address_space(4))) uint32_t *)(uintptr_t)(row + i));
     return p < a.c.pages ? p : kNoPage;
 }
+
+constexpr float kNothing = -3e38f;      // a running maximum before the first score
 
 // ---- which item ------------------------------------------------------------------------------------------------------------------
 struct PagedItem {
@@ -251,6 +253,15 @@ template <bool BF, int N, class Frag> __device__ __forceinline__ void pg_cut(flo
     }
 }
 
+// s * f, rounded, less m
+constexpr float kFar = 1048576.f;
+__device__ __forceinline__ float pg_apart(float s, float f, float m)
+{
+#pragma clang fp contract(off)
+    const float x = s * f;
+    return x - m;
+}
+
 // bits where one of two 16-bit numbers is not finite
 template <bool BF> __device__ __forceinline__ uint32_t pg_special(uint32_t w)
 {
@@ -435,7 +446,7 @@ __global__ __launch_bounds__(256, paged_rows_waves(D, CT, NQ, QT)) void paged_ro
     float m[QT], l[QT];
 #pragma unroll
     for (int i = 0; i < QT; i++) {
-        m[i] = -1e30f;
+        m[i] = kNothing;
         l[i] = 0.f;
 #pragma unroll
         for (int d = 0; d < DT; d++) o[d][i] = pg_f4{0.f, 0.f, 0.f, 0.f};
@@ -748,7 +759,7 @@ __global__ __launch_bounds__(256, paged_rows_waves(D, CT, NQ, QT)) void paged_ro
             float y[8], ms[4];
 #pragma unroll
             for (int e = 0; e < 8; e++) y[e] = 0.f;
-            float big = -1e30f, all = 0.f;
+            float big = kNothing, all = 0.f;
 #pragma unroll
             for (int w = 0; w < 4; w++) {
                 ms[w] = ml[w][i * 16 + row][0];
@@ -982,7 +993,7 @@ __global__ __launch_bounds__(256, 2) void paged_tile_kernel(PagedAttnArgs a)
     for (int d = 0; d < DT; d++)
 #pragma unroll
         for (int i = 0; i < 16; i++) o[d][i] = 0.f;
-    float m = -1e30f, l = 0.f;
+    float m = kNothing, l = 0.f, less = -kNothing;      // less: kLift - m, or what lets the weights overflow
 
     // Which of a tile's four runs of 16 keys have a page?  All of them, unless one of the item's pages is missing: looked up once.
     uint32_t missing = 0;
@@ -1117,20 +1128,20 @@ __global__ __launch_bounds__(256, 2) void paged_tile_kernel(PagedAttnArgs a)
         }
         Frag p[4];      // 16 keys each
         float sum;
-        auto weigh = [&]() {
-            const float less = kLift - m;
+        auto weigh = [&](auto exponent) {
             sum = 0.f;
 #pragma unroll
             for (int j = 0; j < 4; j++)
 #pragma unroll
                 for (int e = 0; e < 8; e++) {
-                    const float w = pg_exp2(fmaf(sc[j / 2][j % 2 * 8 + e], factor, less));
+                    const float w = pg_exp2(exponent(sc[j / 2][j % 2 * 8 + e]));
                     sum += w;
                     if constexpr (BF) p[j][e] = (__bf16)w;
                     else p[j][e] = (_Float16)w;
                 }
         };
-        weigh();
+        const auto near = [&](float s) { return fmaf(s, factor, less); };
+        weigh(near);
         if (__any(!(sum <= MOST))) {      // the reference is too small, as at first; or a score is no number
             float top = -INFINITY;
 #pragma unroll
@@ -1144,7 +1155,11 @@ __global__ __launch_bounds__(256, 2) void paged_tile_kernel(PagedAttnArgs a)
             for (int d = 0; d < DT; d++)
 #pragma unroll
                 for (int i = 0; i < 16; i++) o[d][i] *= f;
-            weigh();
+            // A product and its rounding, the reference, are far apart where they are large: the weights are then those of rounded products, and the row comes here in every tile
+            const bool far = fabsf(m) > kFar;
+            less = far ? -kNothing : kLift - m;
+            if (__any(far)) weigh([&](float s) { return far ? pg_apart(s, factor, m) + kLift : near(s); });
+            else weigh(near);
         }
         l += sum;
 #pragma unroll
@@ -1252,7 +1267,7 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttnArgs a, float 
     // of a row's parts a wave takes every WAVES-th
     constexpr int V = D >= 64 ? D / 64 : 1;
     const bool mine = lane * V < D;
-    float top = -1e30f, all = 0.f, y[V];
+    float top = kNothing, all = 0.f, y[V];
 #pragma unroll
     for (int e = 0; e < V; e++) y[e] = 0.f;
     for (uint32_t p0 = wave - first; cut && p0 < it.parts; p0 += 4 * WAVES) {
@@ -1264,7 +1279,7 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttnArgs a, float 
             ms[j] = a.part_ml[2 * at];
             ls[j] = a.part_ml[2 * at + 1];
             if (p >= it.parts) {
-                ms[j] = -1e30f;
+                ms[j] = kNothing;
                 ls[j] = 0.f;
             }
 #pragma unroll
@@ -1295,7 +1310,7 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttnArgs a, float 
     float big = tops[first][0];
 #pragma unroll
     for (int w = 1; w < WAVES; w++) big = fmaxf(big, tops[first + w][0]);
-    const float sink = a.sinks ? a.sinks[h] * 1.44269504088896341f : -1e30f;
+    const float sink = a.sinks ? a.sinks[h] * 1.44269504088896341f : kNothing;
     big = fmaxf(big, sink);
     float total = a.sinks ? pg_exp2(sink - big + lift) : 0.f, z[8];
 #pragma unroll

@@ -133,7 +133,8 @@ extern "C" int lv_kernel_paged_attention(lv_ctx *c, void *out, uint32_t ldo, con
     if (p.bytes && (!work || work_bytes < p.bytes || (uintptr_t)work % 16))
         return fail(LV_ERR_ARG, "lv_kernel_paged_attention: a workspace of %llu bytes, aligned to 16, is needed", (unsigned long long)p.bytes);
     const uint64_t grid = p.items * cache->kv_heads, rows = (uint64_t)batch->tokens * spec->heads;
-    if (grid > 0x7fffffffu || rows > 0x7fffffffu) return fail(LV_ERR_RANGE, "lv_kernel_paged_attention: %u tokens of %u heads", batch->tokens, spec->heads);
+    // 2^24 workgroups of 256 are more than a launch may have
+    if (grid > 0xffffffu || rows > 0x7fffffffu) return fail(LV_ERR_RANGE, "lv_kernel_paged_attention: %u tokens of %u heads", batch->tokens, spec->heads);
     PagedAttnArgs &a = p.args;
     a.c = paged_view(*cache);
     a.starts = batch->starts;

@@ -153,7 +153,7 @@ inline const char *paged_batch_refusal(const lv_paged_cache *c, const lv_paged_b
     if (!c->data) return "the cache has no data";
     if ((uintptr_t)c->data % 16) return "the cache's data is not aligned to 16 bytes";
     if (b->seqs > 65535) return "more than 65535 sequences";
-    if (b->tokens > (1u << 24)) return "more than 2^24 tokens";
+    if (b->tokens >= (1u << 24)) return "2^24 tokens or more";
     if ((uint64_t)b->table_ld * c->page > (1u << 30)) return "the table covers more than 2^30 positions";
     if (b->seqs && (!b->starts || !b->lens || (!b->table && b->table_ld))) return "starts, lens or table is null";
     if (((uintptr_t)b->starts | (uintptr_t)b->lens | (uintptr_t)b->table) % 4) return "starts, lens or table is not aligned to 4 bytes";
@@ -201,7 +201,7 @@ inline const char *rotate_refusal(const void *out, uint32_t ldo, const void *x, 
     if (!size) return "the type is none of LV_F32, LV_F16, LV_BF16";
     if (dim == 0 || dim > 512 || dim % 8) return "dim is no multiple of 8 from 8 to 512";
     if (heads == 0 || heads > 65536) return "heads is not in 1 .. 65536";
-    if (tokens > (1u << 24)) return "more than 2^24 tokens";
+    if (tokens >= (1u << 24)) return "2^24 tokens or more";
     if (s->rot_dims % 2 || s->rot_dims > dim) return "rot_dims is odd or larger than dim";
     if (s->flags & ~(uint32_t)(LV_ROTATE_HALVES | LV_ROTATE_PER_AXIS)) return "unknown flags";
     if (!(s->rot_base > 0) || !(s->rot_base - s->rot_base == 0)) return "rot_base is not above 0, or not finite";

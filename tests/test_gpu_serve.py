@@ -395,6 +395,44 @@ def test_attention_scales(dev, scale, new):
     assert np.all(np.abs(got - want) <= ref.attention_bound(want, size, reach, seen, mass, 64, F16, F16))
 
 
+@pytest.mark.parametrize("cache,kind,new", [(BF16, F32, 1), (BF16, F32, 40), (BF16, BF16, 1), (BF16, BF16, 60)], ids=str)
+@pytest.mark.parametrize("keys", [100, 600])
+def test_attention_of_scores_far_below_zero(dev, cache, kind, new, keys):
+    """Scores of -10^33 and less: the largest key's has all the weight, 10^27 above the next, so a row is its values, rounded at most twice (pieces, and the quotient)"""
+    rng = np.random.default_rng(53)
+    pool = ref.Pool(cache, 1, 64, 16, 40, rng)
+    step = ref.Step(pool, [keys], [new], rng)
+    v = ref.decode(ref.encode(rng.standard_normal((keys, 64)), BF16), BF16)
+    best = rng.integers(0, keys - new)
+    for p in range(keys):
+        at = step.place(pool, 0, p)
+        pool.put(at[0], 0, 0, at[1], np.full(64, 1e15 if p == best else 1.5e15 + 1e13 * (p % 90)))
+        pool.put(at[0], 0, 1, at[1], v[p])
+    got, held = run_attention(dev, pool, step, np.full((new, 2, 64), -1e17), kind, 2, 0.125)
+    assert np.all(np.abs(got - v[best]) <= 2.0 ** -20 * np.abs(v[best]) if kind == F32 else got == v[best])
+
+
+@pytest.mark.parametrize("cache", [F16, Q4], **KINDS)
+@pytest.mark.parametrize("new", [2, 50])
+def test_attention_of_sequences_that_share_pages(dev, cache, new):
+    """a common beginning is stored once: the same pages in several rows of the table, and one sequence twice"""
+    def edit(pool, step):
+        step.table[1, :25] = step.table[0, :25]
+        step.table[2] = step.table[0]
+        step.lens[2] = step.lens[0]
+    check_attention(dev, np.random.default_rng(54), cache, F16, 4, 2, 64, 16, [500, 470, 500], [new, new, new], edit=edit)
+
+
+def test_attention_of_more_workgroups_than_a_launch_has(dev):
+    """refused before anything is looked at"""
+    lva, ctx = dev.lva, dev.ctx
+    p = dev.put(np.zeros(64, np.uint32))
+    c = lva.PagedCache(p.value, F16, 64, 32, 16, 1)
+    b, spec = lva.PagedBatch(1, (1 << 24) - 1, p.value, p.value, p.value, 1), lva.PagedAttnSpec(64, 1.0, 0, 0, None)
+    with pytest.raises(lva.LvError, match="tokens"):
+        ctx.paged_attention(p, 2048, p, 2048, F16, c, b, spec, p, 1 << 40)
+
+
 @pytest.mark.parametrize("cache", [F16, Q8], **KINDS)
 def test_attention_without_pages(dev, cache):
     """keys whose page is not in the pool are hidden; a row that sees nothing is 0, also beside a sink"""
@@ -601,8 +639,9 @@ class Graph:
         assert self.hip.hipGraphExecDestroy(self.exe) == 0
 
 
+@pytest.mark.parametrize("columns", [12, 30])      # one launch of attention; cut, and put together by a second one
 @pytest.mark.parametrize("cache,kind", [(F16, F32), (BF16, BF16), (Q8, F16), (Q4, BF16)], ids=lambda k: ref.NAMES[k])
-def test_a_step_of_drafts_captured_and_replayed(dev, cache, kind):
+def test_a_step_of_drafts_captured_and_replayed(dev, cache, kind, columns):
     """Queries and keys turned, rows written, attention over all of it, drafts verified: one graph, replayed for several steps whose lengths, pages, rows and random
     numbers change on the device.  Every step against the definitions, on the pool as the device has it."""
     lva, ctx = dev.lva, dev.ctx
@@ -610,7 +649,8 @@ def test_a_step_of_drafts_captured_and_replayed(dev, cache, kind):
     heads, kv_heads, dim, page, seqs, drafts, vocab = 8, 2, 64, 16, 3, 3, 700
     new = drafts + 1
     pool = ref.Pool(cache, kv_heads, dim, page, 40, rng)
-    table = rng.permutation(40)[:36].reshape(seqs, 12).astype(np.uint32)
+    table = np.full((seqs, columns), NO_PAGE, dtype=np.uint32)
+    table[:, :12] = rng.permutation(40)[:36].reshape(seqs, 12)
     lens = np.array([0, 20, 100])
     for s in range(seqs):                 # what the sequences hold already
         for p in range(lens[s]):
@@ -621,9 +661,10 @@ def test_a_step_of_drafts_captured_and_replayed(dev, cache, kind):
     dpool, c = dev.cache(pool)
     starts = (np.arange(seqs + 1) * new).astype(np.uint32)
     dlens, dpos, dqkv = dev.put(np.zeros(seqs, np.uint32)), dev.put(np.zeros(rows, np.uint32)), dev.put(ref.encode(np.zeros((rows, width)), kind))
-    b = lva.PagedBatch(seqs, rows, dev.put(starts).value, dlens.value, dev.put(table).value, 12)
+    b = lva.PagedBatch(seqs, rows, dev.put(starts).value, dlens.value, dev.put(table).value, columns)
     spec, rot = lva.PagedAttnSpec(heads, 0.125, 0, 0, None), lva.RotateSpec(dim, 1e4, (0, 0, 0), lva.ROTATE_HALVES)
     n = ctx.paged_attention_workspace(kind, c, b, spec)
+    assert (n > 0) == (columns > 24)
     work = dev.put(np.zeros(n + 16, np.uint8))
     out = dev.put(ref.encode(np.zeros((rows, heads * dim)), kind))
     size = ref.BYTES[kind]
