@@ -297,6 +297,8 @@ __device__ __forceinline__ pg_s4 pg_read_columns(const uint8_t *p)
 // NQ: pieces of a query, 1, or with 32-bit queries 2 (fp16 rows: 22 bits) or 3 (bf16 rows: 24 bits); the weights have as many, 2 of bf16 at least.  Rows of
 // codes: keys enter as exact integers, a block's sum is scaled in fp32.  Values are scaled in fp16 (a rounding of 2^-11 of each, beside the 16-bit result's own); with
 // 32-bit queries they enter as two fp16 pieces, which hold them exactly: 19 bits at most, the last of them 2^-24 or more, as the scale's is.
+// FINE: rows of codes and an fp16 result.  Its own rounding is no coarser than the weights' and the scaled values' are, and with both the error is 1.6 times the result's
+// rounding alone; the weights enter as two pieces, and it is 1.4 times (single tokens and drafts: 1 to 7 % of the time).  Beside a bf16 result neither shows.
 typedef uint32_t pg_u2 __attribute__((ext_vector_type(2)));
 template <int BYTES> struct PgWord { typedef uint32_t type; };
 template <> struct PgWord<8> { typedef pg_u2 type; };
@@ -309,11 +311,11 @@ constexpr int paged_rows_waves(int D, int CT, int NQ, int QT)
     return NQ > 1 && QT == 2 ? 2 : 3;
 }
 
-template <int D, int CT, int NQ, int QT>
+template <int D, int CT, int NQ, int QT, bool FINE>
 __global__ __launch_bounds__(256, paged_rows_waves(D, CT, NQ, QT)) void paged_rows_kernel(PagedAttnArgs a)
 {
     constexpr bool BF = CT == kPgBf16, BLOCKS = CT == kPgQ8 || CT == kPgQ4, EXACT = NQ > 1;
-    constexpr int KS = D / 32, DT = D / 16, CH = D / 8, ROW = 2 * D + 16, NP = BF && NQ == 1 ? 2 : NQ, TILE = 16 * QT;
+    constexpr int KS = D / 32, DT = D / 16, CH = D / 8, ROW = 2 * D + 16, NP = (BF || FINE) && NQ == 1 ? 2 : NQ, TILE = 16 * QT;
     constexpr float kLift = BF ? 0.f : 12.f, kRoom = 3.f;
     constexpr int MERGE = D + 4;                      // floats of a row of results in LDS
     typedef typename PgFrag<BF>::type Frag;
@@ -802,6 +804,7 @@ __global__ __launch_bounds__(256, paged_rows_waves(D, CT, NQ, QT)) void paged_ro
 // The running maximum is a reference: weights are formed with it at once, and only where their sum says that a score is far above it are the maximum taken, the results
 // rescaled and the weights formed anew.  Most tiles do without the maximum's 48 vector instructions (half of them make numbers canonical).
 // Weights enter the second product as one fp16 (2^-11) or bf16 (2^-8) number: beside a 16-bit result's own rounding, over all the keys of a row.
+// FINE: as two fp16 pieces, as above (1024 tokens behind four times as many keys, 8 bits: 128 and 165 us; 4 bits 125 and 157).
 typedef float pg_f16v __attribute__((ext_vector_type(16)));
 
 
@@ -832,7 +835,7 @@ template <int N> __device__ __forceinline__ void pg_load_direct(uint32_t to, con
 constexpr int kPagedTileRows = 128;
 constexpr float paged_tile_lift(bool bf) { return bf ? 0.f : 6.f; }      // of the weight of a score at the reference, log2
 
-template <int D, int CT>
+template <int D, int CT, bool FINE>
 __global__ __launch_bounds__(256, 2) void paged_tile_kernel(PagedAttnArgs a)
 {
     constexpr bool BF = CT == kPgBf16, BLOCKS = CT == kPgQ8 || CT == kPgQ4;
@@ -1126,7 +1129,7 @@ __global__ __launch_bounds__(256, 2) void paged_tile_kernel(PagedAttnArgs a)
                     sc[kt][i] = first + (32 * kt + 8 * (i / 4) + i % 4) < sees ? sc[kt][i] : -INFINITY;
                 }
         }
-        Frag p[4];      // 16 keys each
+        Frag p[4], rest[FINE ? 4 : 1];      // 16 keys each
         float sum;
         auto weigh = [&](auto exponent) {
             sum = 0.f;
@@ -1136,8 +1139,13 @@ __global__ __launch_bounds__(256, 2) void paged_tile_kernel(PagedAttnArgs a)
                 for (int e = 0; e < 8; e++) {
                     const float w = pg_exp2(exponent(sc[j / 2][j % 2 * 8 + e]));
                     sum += w;
-                    if constexpr (BF) p[j][e] = (__bf16)w;
-                    else p[j][e] = (_Float16)w;
+                    if constexpr (BF) {
+                        p[j][e] = (__bf16)w;
+                    } else {
+                        const _Float16 h = (_Float16)w;
+                        p[j][e] = h;
+                        if constexpr (FINE) rest[j][e] = (_Float16)(w - (float)h);
+                    }
                 }
         };
         const auto near = [&](float s) { return fmaf(s, factor, less); };
@@ -1165,7 +1173,11 @@ __global__ __launch_bounds__(256, 2) void paged_tile_kernel(PagedAttnArgs a)
 #pragma unroll
         for (int j = 0; j < 4; j++)
 #pragma unroll
-            for (int d = 0; d < DT; d++) o[d] = pg_mfma32<BF>(values(vt_lds, d, j), p[j], o[d]);
+            for (int d = 0; d < DT; d++) {
+                const Frag v = values(vt_lds, d, j);
+                if constexpr (FINE) o[d] = pg_mfma32<BF>(v, rest[j], o[d]);
+                o[d] = pg_mfma32<BF>(v, p[j], o[d]);
+            }
         finish();
     }
     __syncthreads();

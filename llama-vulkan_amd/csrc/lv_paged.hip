@@ -70,39 +70,42 @@ AttnPlan attn_plan(uint32_t units, uint32_t type, const lv_paged_cache &c, const
     return p;
 }
 
-template <int D, int CT, int NQ>
+template <int D, int CT, int NQ, bool FINE = false>
 void launch_rows(const AttnPlan &p, uint32_t grid, hipStream_t st)
 {
     if constexpr (D <= 128) {
         if (p.tiles == 2) {
-            paged_rows_kernel<D, CT, NQ, 2><<<dim3(grid), dim3(256), 0, st>>>(p.args);
+            paged_rows_kernel<D, CT, NQ, 2, FINE><<<dim3(grid), dim3(256), 0, st>>>(p.args);
             return;
         }
     }
-    paged_rows_kernel<D, CT, NQ, 1><<<dim3(grid), dim3(256), 0, st>>>(p.args);
+    paged_rows_kernel<D, CT, NQ, 1, FINE><<<dim3(grid), dim3(256), 0, st>>>(p.args);
 }
+
+template <int D, int CT, bool FINE>
+void launch_tiles(const PagedAttnArgs &a, uint32_t grid, hipStream_t st) { paged_tile_kernel<D, CT, FINE><<<dim3(grid), dim3(256), 0, st>>>(a); }
 
 template <int D>
 void launch_attention(const AttnPlan &p, uint32_t grid, hipStream_t st)
 {
     const PagedAttnArgs &a = p.args;
-    const bool bf = a.c.type == LV_BF16;
+    const bool bf = a.c.type == LV_BF16, fine = a.type == LV_F16;
     float lift = bf ? 0.f : 12.f;
     if (p.tiles == 8) {
         lift = paged_tile_lift(bf);
         if constexpr (D == 64 || D == 128) {
             switch (a.c.type) {
-            case LV_F16: paged_tile_kernel<D, kPgF16><<<dim3(grid), dim3(256), 0, st>>>(a); break;
-            case LV_BF16: paged_tile_kernel<D, kPgBf16><<<dim3(grid), dim3(256), 0, st>>>(a); break;
-            case LV_Q8_0: paged_tile_kernel<D, kPgQ8><<<dim3(grid), dim3(256), 0, st>>>(a); break;
-            default: paged_tile_kernel<D, kPgQ4><<<dim3(grid), dim3(256), 0, st>>>(a); break;
+            case LV_F16: launch_tiles<D, kPgF16, false>(a, grid, st); break;
+            case LV_BF16: launch_tiles<D, kPgBf16, false>(a, grid, st); break;
+            case LV_Q8_0: fine ? launch_tiles<D, kPgQ8, true>(a, grid, st) : launch_tiles<D, kPgQ8, false>(a, grid, st); break;
+            default: fine ? launch_tiles<D, kPgQ4, true>(a, grid, st) : launch_tiles<D, kPgQ4, false>(a, grid, st); break;
             }
         }
     } else switch (a.c.type) {
     case LV_F16: p.pieces == 1 ? launch_rows<D, kPgF16, 1>(p, grid, st) : launch_rows<D, kPgF16, 2>(p, grid, st); break;
     case LV_BF16: p.pieces == 1 ? launch_rows<D, kPgBf16, 1>(p, grid, st) : launch_rows<D, kPgBf16, 3>(p, grid, st); break;
-    case LV_Q8_0: p.pieces == 1 ? launch_rows<D, kPgQ8, 1>(p, grid, st) : launch_rows<D, kPgQ8, 2>(p, grid, st); break;
-    default: p.pieces == 1 ? launch_rows<D, kPgQ4, 1>(p, grid, st) : launch_rows<D, kPgQ4, 2>(p, grid, st); break;
+    case LV_Q8_0: p.pieces == 1 ? (fine ? launch_rows<D, kPgQ8, 1, true>(p, grid, st) : launch_rows<D, kPgQ8, 1>(p, grid, st)) : launch_rows<D, kPgQ8, 2>(p, grid, st); break;
+    default: p.pieces == 1 ? (fine ? launch_rows<D, kPgQ4, 1, true>(p, grid, st) : launch_rows<D, kPgQ4, 1>(p, grid, st)) : launch_rows<D, kPgQ4, 2>(p, grid, st); break;
     }
     if (!a.deal.target) return;
     const uint32_t rows = a.deal.tokens * a.deal.group * a.deal.kv_heads;
