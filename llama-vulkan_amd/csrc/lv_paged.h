@@ -306,7 +306,7 @@ template <> struct PgWord<8> { typedef pg_u2 type; };
 constexpr int paged_rows_waves(int D, int CT, int NQ, int QT)
 {
     if (D == 256) return 1;
-    if (D == 128 && QT == 2 && NQ == 3) return 1;      // 59 registers in memory cost more than a second wave gains (1024 tokens behind 3072: 340 us and 281)
+    if (D == 128 && QT == 2 && NQ == 3) return 1;      // 59 registers in memory cost more than a second wave gains (1024 tokens, the last of 4096: 340 us and 281)
     if (D == 128) return QT == 1 && NQ == 1 && CT >= kPgQ8 ? 3 : 2;
     return NQ > 1 && QT == 2 ? 2 : 3;
 }
@@ -825,7 +825,7 @@ template <int N> __device__ __forceinline__ void pg_load_direct(uint32_t to, con
     static_assert(N == 2 || N == 4, "runs");
     if constexpr (N == 4)
         asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %5\n\tglobal_load_lds_dwordx4 %2, %5 offset:1024\n\t"
-                     "global_load_lds_dwordx4 %3, %5 offset:2048\n\tglobal_load_lds_dwordx4 %4, %5 offset:3072"
+                     "global_load_lds_dwordx4 %3, %5 offset:2048\n\tglobal_load_lds_dwordx4 %4, %5 offset:0xc00"
                      : : "s"(__builtin_amdgcn_readfirstlane(to)), "v"(at[0]), "v"(at[1]), "v"(at[2]), "v"(at[3]), "s"(base) : "memory");
     else
         asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %3\n\tglobal_load_lds_dwordx4 %2, %3 offset:1024"
