@@ -357,7 +357,8 @@ int lv_kernel_attention_static(lv_ctx *ctx, float *out, const void *kcache, cons
  *      they read on the device (lengths, pages, ...) may change between replays.  A workspace is written before it is read; two calls that
  *      can overlap, as two captured graphs can, each need one of their own.
  *      Row strides (ld*) count elements.  The pool, workspaces and the rows of q, k, v, x and out (pointer and stride in bytes) are aligned to 16 bytes,
- *      everything else to 4.  The calls leave the caller's current device as it was. */
+ *      everything else to 4.  What a call writes overlaps nothing else that it reads or writes, but for out and x of lv_kernel_rotate.  The calls leave the caller's
+ *      current device as it was. */
 
 /* the stream all work of a context runs on (a hipStream_t, non-blocking), for callers that order other work with it or capture it */
 int lv_ctx_stream(const lv_ctx *ctx, void **stream);

@@ -423,6 +423,37 @@ def test_attention_of_sequences_that_share_pages(dev, cache, new):
     check_attention(dev, np.random.default_rng(54), cache, F16, 4, 2, 64, 16, [500, 470, 500], [new, new, new], edit=edit)
 
 
+@pytest.mark.parametrize("cache,kind", [(F16, F16), (Q8, BF16), (BF16, F32)], ids=str)
+@pytest.mark.parametrize("window,chunk,sinks", [(5, 0, True), (300, 0, False), (0, 50, False), (0, 400, True), (333, 256, True)], ids=str)
+def test_attention_masks_of_calls_that_are_cut(dev, cache, kind, window, chunk, sinks):
+    check_attention(dev, np.random.default_rng(55), cache, kind, 4, 2, 64, 16, [700, 450, 33], [2, 1, 3], window=window, chunk=chunk, sinks=sinks)
+    check_attention(dev, np.random.default_rng(56), cache, kind, 4, 2, 64, 32, [700, 450], [40, 70], window=window, chunk=chunk, sinks=sinks)
+
+
+@pytest.mark.parametrize("cache,kind", [(F16, F16), (Q4, BF16), (F16, F32)], ids=str)
+@pytest.mark.parametrize("new", [1, 3])
+def test_attention_of_many_heads_over_one(dev, cache, kind, new):
+    """a token's heads fill more than a tile: tiles begin in the middle of a token"""
+    check_attention(dev, np.random.default_rng(57), cache, kind, 150, 1, 64, 16, [500, 20, 3], [new, 2, 0], sinks=True, pad=1)
+
+
+def test_a_table_without_columns(dev):
+    """no position has a page: nothing is written or read back, and every row is 0"""
+    lva, ctx = dev.lva, dev.ctx
+    rng = np.random.default_rng(58)
+    pool = ref.Pool(F16, 1, 64, 16, 4, rng)
+    dpool, c = dev.cache(pool)
+    b = lva.PagedBatch(1, 5, dev.put(np.array([0, 5], np.uint32)).value, dev.put(np.array([5], np.uint32)).value, None, 0)
+    x = dev.put(rng.standard_normal((5, 64)).astype(np.float16))
+    y = np.full((5, 64), 7.5, np.float16)
+    out, dk = dev.put(y), dev.put(y)
+    ctx.paged_write(c, b, x, 64, x, 64, F16)
+    ctx.paged_read(c, b, dk, 64, dk, 64, F16)
+    ctx.paged_attention(out, 64, x, 64, F16, c, b, lva.PagedAttnSpec(1, 0.1, 0, 0, None))
+    assert np.array_equal(dev.get(dpool, pool.bytes.shape, np.uint8), pool.bytes) and np.array_equal(dev.get(dk, y.shape, np.float16), y)
+    assert not dev.get(out, y.shape, np.float16).any()
+
+
 def test_attention_of_more_workgroups_than_a_launch_has(dev):
     """refused before anything is looked at"""
     lva, ctx = dev.lva, dev.ctx
