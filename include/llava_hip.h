@@ -450,7 +450,8 @@ typedef struct {
     const float *uniforms;           /* [seqs][drafts + 1], in 0 .. 1, 1 excluded */
 } lv_draft_batch;
 enum { LV_NO_TOKEN = 0xffffffffu };
-/* tokens: [seqs][drafts + 1], the drafts that stand, the next token, LV_NO_TOKEN behind it; accepted: [seqs], how many drafts stand */
+/* tokens: [seqs][drafts + 1], the drafts that stand, the next token, LV_NO_TOKEN behind it; accepted: [seqs], how many drafts stand.
+ * `work`: lv_verify_drafts_workspace bytes, null where that is 0 */
 int lv_verify_drafts_workspace(lv_ctx *ctx, const lv_draft_batch *batch, uint64_t *bytes);
 int lv_kernel_verify_drafts(lv_ctx *ctx, uint32_t *tokens, uint32_t *accepted, const lv_draft_batch *batch, void *work, uint64_t work_bytes);
 

@@ -7,7 +7,8 @@ namespace lv {
 
 // ---- rotary positions --------------------------------------------------------------------------------------------------------------
 // A workgroup turns some heads of one token: the angles are the same for all heads, so they are formed once (in turns, in double, reduced to half a turn before
-// they become fp32: a position of 10^5 leaves nothing of a 32-bit angle) and read from LDS by every head.  Bound by the bytes of x and out.
+// they become fp32: a position of 10^5 leaves nothing of a 32-bit angle) and read from LDS by every head.  Bound by the bytes of x and out
+// (6001 tokens of 40 heads of 128, bf16: 21 us, 5.8 TB/s, part of it from the last cache); one token by its launch (2.7).
 struct RotateArgs {
     const void *x;
     void *out;
@@ -283,7 +284,7 @@ __global__ __launch_bounds__(256) void paged_copy_kernel(PagedRowsArgs a, uint32
 
 // ---- verification of drafts ------------------------------------------------------------------------------------------------------------
 // Two launches: the weights' sums over segments of the row that decides, many workgroups a sequence; then the segment that the random number falls into,
-// a workgroup a sequence.  Sums in double: a running sum of 10^5 floats in 32 bits is off by more than the smallest probabilities.
+// a workgroup a sequence (48 sequences, 7 drafts, 128256 entries: 11 us, 4.1 TB/s, and 4.5; segments of 4096 entries a microsecond more in all).  Sums in double: a running sum of 10^5 floats in 32 bits is off by more than the smallest probabilities.
 struct VerifyArgs {
     lv_draft_batch b;
     uint32_t *tokens, *accepted;
@@ -353,6 +354,39 @@ __device__ __forceinline__ double wave_sum_double(double v)
     return v;
 }
 
+// what is left of the target after the draft, and the target, summed up by a wave whose lanes take entries j .. j + 3 and so on, `step` further each time; AHEAD of them
+// asked for at once
+template <int AHEAD> __device__ __forceinline__ void verify_sums(const VerifyRow &row, uint32_t j, uint32_t end, uint32_t step, double &rest, double &whole)
+{
+    auto add = [&](uint32_t at, const float (&p)[4], const float (&q)[4]) {
+#pragma unroll
+        for (uint32_t e = 0; e < 4; e++) {
+            rest += verify_rest(row.x, at + e, p[e], q[e]);
+            whole += verify_whole(p[e]);
+        }
+    };
+    if (row.wide) {
+        for (; j + (AHEAD - 1) * step + 4 <= end; j += AHEAD * step) {
+            float p[AHEAD][4], q[AHEAD][4];
+#pragma unroll
+            for (int n = 0; n < AHEAD; n++) {
+                const float4 x = *reinterpret_cast<const float4 *>(row.p + j + n * step), y = row.q ? *reinterpret_cast<const float4 *>(row.q + j + n * step) : make_float4(0.f, 0.f, 0.f, 0.f);
+                p[n][0] = x.x; p[n][1] = x.y; p[n][2] = x.z; p[n][3] = x.w;
+                q[n][0] = y.x; q[n][1] = y.y; q[n][2] = y.z; q[n][3] = y.w;
+            }
+#pragma unroll
+            for (int n = 0; n < AHEAD; n++) add(j + n * step, p[n], q[n]);
+        }
+    }
+    for (; j < end; j += step) {
+        float p[4], q[4];
+        verify_load4(row, j, end, p, q);
+        add(j, p, q);
+    }
+    rest = wave_sum_double(rest);
+    whole = wave_sum_double(whole);
+}
+
 // grid (segments, seqs)
 __global__ __launch_bounds__(256) void verify_sums_kernel(VerifyArgs a)
 {
@@ -363,18 +397,7 @@ __global__ __launch_bounds__(256) void verify_sums_kernel(VerifyArgs a)
     const VerifyRow row = verify_row(a.b, seq, r, count);
     if (blockIdx.x == 0 && threadIdx.x == 0) a.accepted[seq] = r;
     double rest = 0.0, whole = 0.0;
-#pragma unroll 2
-    for (uint32_t j = j0 + 4 * threadIdx.x; j < j1; j += 1024) {
-        float p[4], q[4];
-        verify_load4(row, j, j1, p, q);
-#pragma unroll
-        for (uint32_t e = 0; e < 4; e++) {
-            rest += verify_rest(row.x, j + e, p[e], q[e]);
-            whole += verify_whole(p[e]);
-        }
-    }
-    rest = wave_sum_double(rest);
-    whole = wave_sum_double(whole);
+    verify_sums<2>(row, j0 + 4 * threadIdx.x, j1, 1024, rest, whole);
     if ((threadIdx.x & 63) == 0) {
         part[threadIdx.x >> 6][0] = rest;
         part[threadIdx.x >> 6][1] = whole;
@@ -383,17 +406,13 @@ __global__ __launch_bounds__(256) void verify_sums_kernel(VerifyArgs a)
     if (threadIdx.x < 2) a.sums[((uint64_t)seq * a.segments + blockIdx.x) * 2 + threadIdx.x] = (part[0][threadIdx.x] + part[1][threadIdx.x]) + (part[2][threadIdx.x] + part[3][threadIdx.x]);
 }
 
-// grid (seqs).  `accepted` is what the sums' launch found
-__global__ __launch_bounds__(256) void verify_pick_kernel(VerifyArgs a)
+// The token of the row, and all tokens of the sequence.  By a workgroup, the first 256 threads of it do the work; rest and whole: the segments' sums, by lane in every wave
+__device__ __forceinline__ void verify_pick(const VerifyArgs &a, uint32_t seq, uint32_t r, const VerifyRow &row, double rest, double whole)
 {
     __shared__ double waves[4];
     __shared__ uint32_t found, last;
-    const uint32_t seq = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const uint32_t r = a.accepted[seq], count = a.b.counts ? min(a.b.counts[seq], a.b.drafts) : a.b.drafts;
-    const VerifyRow row = verify_row(a.b, seq, r, count);
-    // segments, 64 at most: running sums by lane
-    const bool mine = lane < a.segments;
-    const double rest = mine ? a.sums[((uint64_t)seq * a.segments + lane) * 2] : 0.0, whole = mine ? a.sums[((uint64_t)seq * a.segments + lane) * 2 + 1] : 0.0;
+    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const bool mine = lane < a.segments, works = threadIdx.x < 256;
     const bool use_rest = wave_sum_double(rest) > 0.0;
     double upto = use_rest ? rest : whole;
     const double own = upto;
@@ -422,7 +441,7 @@ __global__ __launch_bounds__(256) void verify_pick_kernel(VerifyArgs a)
 #pragma unroll
             for (uint32_t h = 0; h < 2; h++) {
                 float p[4], q[4];
-                verify_load4(row, min(from + 4 * h, j1), j1, p, q);
+                verify_load4(row, works ? min(from + 4 * h, j1) : j1, j1, p, q);
 #pragma unroll
                 for (uint32_t e = 0; e < 4; e++) w[4 * h + e] = use_rest ? verify_rest(row.x, from + 4 * h + e, p[e], q[e]) : verify_whole(p[e]);
             }
@@ -437,10 +456,10 @@ __global__ __launch_bounds__(256) void verify_pick_kernel(VerifyArgs a)
                 const double v = __shfl_up(run, off, 64);
                 if (lane >= (uint32_t)off) run += v;
             }
-            if (lane == 63) waves[wave] = run;
+            if (lane == 63 && works) waves[wave] = run;
             __syncthreads();
             double start = before;
-            for (uint32_t v = 0; v < wave; v++) start += waves[v];
+            for (uint32_t v = 0; v < min(wave, 4u); v++) start += waves[v];
             const double all = before + ((waves[0] + waves[1]) + (waves[2] + waves[3]));
             run += start;
             const uint64_t first = __ballot((run > goal) & (sum > 0.0)), holds = __ballot(some != 0xffffffffu);
@@ -469,6 +488,39 @@ __global__ __launch_bounds__(256) void verify_pick_kernel(VerifyArgs a)
         const uint32_t i = threadIdx.x;
         a.tokens[(uint64_t)seq * (a.b.drafts + 1) + i] = i < r ? a.b.tokens[(uint64_t)seq * a.b.drafts + i] : i == r ? pick : (uint32_t)LV_NO_TOKEN;
     }
+}
+
+// grid (seqs).  `accepted` is what the sums' launch found
+__global__ __launch_bounds__(256) void verify_pick_kernel(VerifyArgs a)
+{
+    const uint32_t seq = blockIdx.x, lane = threadIdx.x & 63;
+    const uint32_t r = a.accepted[seq], count = a.b.counts ? min(a.b.counts[seq], a.b.drafts) : a.b.drafts;
+    const bool mine = lane < a.segments;      // 64 at most
+    const double rest = mine ? a.sums[((uint64_t)seq * a.segments + lane) * 2] : 0.0, whole = mine ? a.sums[((uint64_t)seq * a.segments + lane) * 2 + 1] : 0.0;
+    verify_pick(a, seq, r, verify_row(a.b, seq, r, count), rest, whole);
+}
+
+// Both at once, a segment for each of 16 waves.  Bound by a chain of loads (drafts, their probabilities, rows, the segment again), then by a compute unit's vector work
+// in double: 8 us a call of one sequence of 8192 entries, 9.8 of 32000, 26 of 128256.  grid (seqs)
+__global__ __launch_bounds__(1024) void verify_whole_kernel(VerifyArgs a)
+{
+    __shared__ double sums[16][2];
+    const uint32_t seq = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    uint32_t count;
+    const uint32_t r = verify_standing(a.b, seq, count);
+    const VerifyRow row = verify_row(a.b, seq, r, count);
+    double rest = 0.0, whole = 0.0;
+    verify_sums<4>(row, wave * a.length + 4 * lane, min((wave + 1) * a.length, a.b.vocab), 256, rest, whole);
+    if (lane == 0) {
+        sums[wave][0] = rest;
+        sums[wave][1] = whole;
+    }
+    __syncthreads();
+    const bool mine = lane < a.segments;
+    rest = mine ? sums[lane][0] : 0.0;
+    whole = mine ? sums[lane][1] : 0.0;
+    if (threadIdx.x == 0) a.accepted[seq] = r;
+    verify_pick(a, seq, r, row, rest, whole);
 }
 
 }  // namespace lv

@@ -103,13 +103,18 @@ extern "C" int lv_kernel_paged_read(lv_ctx *c, const lv_paged_cache *cache, cons
     return paged_copy("lv_kernel_paged_read", false, c, cache, batch, k, ldk, v, ldv, type);
 }
 
+// Few and short rows are one launch, a workgroup a sequence.  us, one launch and two, of 1, 16 and 48 sequences: 8192 entries 8.1 11.2, 8.1 11.1, 8.1 11.1; 32000 9.8 11.3,
+// 10.1 11.0, 11.8 11.1; 50000 12.4 11.1, 15.8 11.1, 16.6 11.2
+static bool verify_one(const lv_draft_batch &b) { return (b.vocab <= 16384 && b.seqs <= 256) || (b.vocab <= 32768 && b.seqs <= 16); }
+
 // entries of a segment, and segments
 static void verify_segments(const lv_draft_batch &b, uint32_t &length, uint32_t &segments)
 {
-    segments = std::min(kVerifySegments, (b.vocab + kVerifySegment - 1) / kVerifySegment);
+    segments = verify_one(b) ? 16 : std::min(kVerifySegments, (b.vocab + kVerifySegment - 1) / kVerifySegment);
     length = ((b.vocab + segments - 1) / segments + 255) / 256 * 256;
     segments = (b.vocab + length - 1) / length;
 }
+static uint64_t verify_bytes(const lv_draft_batch &b, uint32_t segments) { return verify_one(b) ? 0 : (uint64_t)b.seqs * segments * 2 * sizeof(double); }
 
 extern "C" int lv_verify_drafts_workspace(lv_ctx *c, const lv_draft_batch *batch, uint64_t *bytes)
 {
@@ -119,7 +124,7 @@ extern "C" int lv_verify_drafts_workspace(lv_ctx *c, const lv_draft_batch *batch
     if (!c) return fail(LV_ERR_ARG, "lv_verify_drafts_workspace: ctx is null");
     uint32_t length, segments;
     verify_segments(*batch, length, segments);
-    *bytes = (uint64_t)batch->seqs * segments * 2 * sizeof(double);
+    *bytes = verify_bytes(*batch, segments);
     return LV_OK;
 }
 
@@ -134,15 +139,19 @@ extern "C" int lv_kernel_verify_drafts(lv_ctx *c, uint32_t *tokens, uint32_t *ac
     a.tokens = tokens;
     a.accepted = accepted;
     verify_segments(*batch, a.length, a.segments);
-    const uint64_t bytes = (uint64_t)batch->seqs * a.segments * 2 * sizeof(double);
-    if (!work || work_bytes < bytes || (uintptr_t)work % 16)
+    const uint64_t bytes = verify_bytes(*batch, a.segments);
+    if (bytes && (!work || work_bytes < bytes || (uintptr_t)work % 16))
         return fail(LV_ERR_ARG, "lv_kernel_verify_drafts: a workspace of %llu bytes, aligned to 16, is needed", (unsigned long long)bytes);
     a.sums = static_cast<double *>(work);
     DeviceScope scope(ctx_device(c));
     HIP_TRY(scope.error);
     const hipStream_t st = ctx_stream(c);
-    verify_sums_kernel<<<dim3(a.segments, batch->seqs), dim3(256), 0, st>>>(a);
-    verify_pick_kernel<<<dim3(batch->seqs), dim3(256), 0, st>>>(a);
+    if (!bytes) {
+        verify_whole_kernel<<<dim3(batch->seqs), dim3(1024), 0, st>>>(a);
+    } else {
+        verify_sums_kernel<<<dim3(a.segments, batch->seqs), dim3(256), 0, st>>>(a);
+        verify_pick_kernel<<<dim3(batch->seqs), dim3(256), 0, st>>>(a);
+    }
     HIP_TRY(hipGetLastError());
     return LV_OK;
 }

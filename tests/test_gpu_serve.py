@@ -570,7 +570,8 @@ def run_verify(dev, target, draft, tokens, counts, uniforms, pad=3):
 
 
 @pytest.mark.parametrize("sampled", [True, False])
-@pytest.mark.parametrize("seqs,drafts,vocab", [(1, 1, 1), (3, 2, 2), (1, 4, 32000), (40, 7, 513), (9, 64, 100), (2, 3, 128256), (5, 5, 2049), (70, 1, 256)])
+@pytest.mark.parametrize("seqs,drafts,vocab", [(1, 1, 1), (3, 2, 2), (1, 4, 32000), (40, 7, 513), (9, 64, 100), (2, 3, 128256), (5, 5, 2049), (70, 1, 256), (300, 2, 513), (16, 1, 32768),
+                                               (17, 1, 16385), (1, 2, 33001)])
 def test_verify(dev, seqs, drafts, vocab, sampled):
     rng = np.random.default_rng(51)
     target = probabilities(rng, (seqs, drafts + 1, vocab))
@@ -638,7 +639,8 @@ def test_verified_tokens_follow_the_target(dev):
 def test_verify_workspace_refusals(dev):
     lva, ctx = dev.lva, dev.ctx
     p = dev.put(np.zeros(4096, np.float32))
-    b = lva.DraftBatch(1, 1, 1000, p.value, 1000, None, 0, p.value, None, p.value)
+    assert ctx.verify_drafts_workspace(lva.DraftBatch(1, 1, 1000, p.value, 1000, None, 0, p.value, None, p.value)) == 0      # one launch
+    b = lva.DraftBatch(1, 1, 40000, p.value, 40000, None, 0, p.value, None, p.value)
     n = ctx.verify_drafts_workspace(b)
     for w, size in ((None, n), (p, n - 1), (p.value + 8, n)):
         with pytest.raises(lva.LvError, match="workspace"):
@@ -670,14 +672,14 @@ class Graph:
         assert self.hip.hipGraphExecDestroy(self.exe) == 0
 
 
-@pytest.mark.parametrize("columns", [12, 30])      # one launch of attention; cut, and put together by a second one
+@pytest.mark.parametrize("columns", [12, 30])      # one launch of attention and of verification; two of each
 @pytest.mark.parametrize("cache,kind", [(F16, F32), (BF16, BF16), (Q8, F16), (Q4, BF16)], ids=lambda k: ref.NAMES[k])
 def test_a_step_of_drafts_captured_and_replayed(dev, cache, kind, columns):
     """Queries and keys turned, rows written, attention over all of it, drafts verified: one graph, replayed for several steps whose lengths, pages, rows and random
     numbers change on the device.  Every step against the definitions, on the pool as the device has it."""
     lva, ctx = dev.lva, dev.ctx
     rng = np.random.default_rng(61)
-    heads, kv_heads, dim, page, seqs, drafts, vocab = 8, 2, 64, 16, 3, 3, 700
+    heads, kv_heads, dim, page, seqs, drafts, vocab = 8, 2, 64, 16, 3, 3, 700 if columns == 12 else 33000
     new = drafts + 1
     pool = ref.Pool(cache, kv_heads, dim, page, 40, rng)
     table = np.full((seqs, columns), NO_PAGE, dtype=np.uint32)
