@@ -311,6 +311,16 @@ def test_attention_of_many_sequences(dev):
     check_attention(dev, rng, F16, F16, 2, 1, 64, 16, lens.tolist(), np.minimum(lens, rng.integers(0, 3, 150)).tolist())
 
 
+@pytest.mark.parametrize("columns", [4, 40])
+def test_attention_of_hundreds_of_sequences(dev, columns):
+    """looked at 256 at a time; where the table covers more than 384 positions, the longest of them are cut"""
+    rng = np.random.default_rng(59)
+    lens = rng.integers(0, 40, 700)
+    lens[[5, 300, 699]] = 600 if columns > 4 else 64
+    new = np.minimum(lens, rng.integers(0, 3, 700))
+    check_attention(dev, rng, F16, F16, 2, 1, 64, 16, lens.tolist(), new.tolist(), pad=2)
+
+
 @pytest.mark.parametrize("cache", [F16, BF16, Q8, Q4], **KINDS)
 def test_attention_of_large_scores(dev, cache):
     """one key takes nearly all weight: 2^-100 and less for the others"""
