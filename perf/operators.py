@@ -187,6 +187,8 @@ def _pool(c, g, dev):
 
 
 def prepare(case, seed):
+    if own:      # the calls run on their context's stream: a program that mixes them with torch's work makes it torch's stream too, once
+        torch.cuda.set_stream(_framework().stream)
     c, dev = case, torch.device("cuda", torch.cuda.current_device())
     g = torch.Generator(device=dev)
     g.manual_seed(seed * 1000003 + 17)
@@ -366,19 +368,28 @@ def _verify(s):
 _kept = {}
 
 
+class _Framework:
+    """the package, a context of it on a device, the context's stream as torch knows it, and a workspace that grows"""
+
+    def __init__(self, device):
+        self.lva = importlib.import_module("llama-vulkan_amd")
+        self.ctx = self.lva.Context(device)
+        self.stream = torch.cuda.ExternalStream(self.ctx.stream(), device=device)
+        self.work = torch.empty(0, dtype=torch.uint8, device=torch.device("cuda", device))
+
+    def workspace(self, size):
+        if self.work.numel() < size:
+            self.ctx.sync()
+            self.work = torch.empty(size, dtype=torch.uint8, device=self.work.device)
+        return self.work.data_ptr()
+
+
 def _framework():
-    """the package, a context of it, and a workspace that grows"""
-    if not _kept:
-        lva = importlib.import_module("llama-vulkan_amd")
-        _kept.update(lva=lva, ctx=lva.Context(torch.cuda.current_device()), work=torch.empty(0, dtype=torch.uint8, device="cuda"))
-    return _kept["lva"], _kept["ctx"]
-
-
-def _workspace(size):
-    if _kept["work"].numel() < size:
-        _kept["ctx"].sync()
-        _kept["work"] = torch.empty(size, dtype=torch.uint8, device="cuda")
-    return _kept["work"].data_ptr()
+    """the current device's"""
+    device = torch.cuda.current_device()
+    if device not in _kept:
+        _kept[device] = _Framework(device)
+    return _kept[device]
 
 
 def _type(lva, name):
@@ -386,7 +397,21 @@ def _type(lva, name):
 
 
 def _own(s):
-    lva, ctx = _framework()
+    """The calls, in order with the current stream's work: as they are where the program has made the context's stream the current one, by events where it has not."""
+    f, here = _framework(), torch.cuda.current_stream()
+    if here == f.stream:
+        return _calls(f, s)
+    f.stream.wait_stream(here)
+    with torch.cuda.stream(f.stream):
+        out = _calls(f, s)
+    here.wait_stream(f.stream)
+    for x in (out,) if isinstance(out, torch.Tensor) else out:
+        x.record_stream(here)
+    return out
+
+
+def _calls(f, s):
+    lva, ctx = f.lva, f.ctx
     c, dev = s["c"], torch.device("cuda", torch.cuda.current_device())
     if c["kind"] == "rotate":
         x, width = s["x"], c["heads"] * c["dim"]
@@ -400,7 +425,7 @@ def _own(s):
         batch = lva.DraftBatch(b, k, c["vocab"], s["target"].data_ptr(), c["vocab"], s["draft"].data_ptr() if s["draft"] is not None else None, c["vocab"],
                                s["tokens"].data_ptr(), s["counts"].data_ptr() if s["counts"] is not None else None, s["uniform"].data_ptr())
         size = ctx.verify_drafts_workspace(batch)
-        ctx.verify_drafts(tokens.data_ptr(), accepted.data_ptr(), batch, _workspace(size), size)
+        ctx.verify_drafts(tokens.data_ptr(), accepted.data_ptr(), batch, f.workspace(size), size)
         return tokens, accepted
     cache = lva.PagedCache(s["pool"].data_ptr(), _type(lva, c["cache"]), c["kv_heads"], c["dim"], c["page"], s["pages"])
     batch = lva.PagedBatch(c["seqs"], s["rows"], s["starts"].data_ptr(), s["lens"].data_ptr(), s["table"].data_ptr(), s["table"].shape[1])
@@ -409,7 +434,7 @@ def _own(s):
         out = torch.empty_like(s["q"])
         spec = lva.PagedAttnSpec(c["heads"], 1 / math.sqrt(c["dim"]), c["window"], 0, s["sinks"].data_ptr() if c["sinks"] else None)
         size = ctx.paged_attention_workspace(t, cache, batch, spec)
-        ctx.paged_attention(out.data_ptr(), out.stride(0), s["q"].data_ptr(), s["q"].stride(0), t, cache, batch, spec, _workspace(size), size)
+        ctx.paged_attention(out.data_ptr(), out.stride(0), s["q"].data_ptr(), s["q"].stride(0), t, cache, batch, spec, f.workspace(size), size)
         return out
     width = c["kv_heads"] * c["dim"]
     if c["kind"] == "store":
