@@ -13,7 +13,7 @@ PATH = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))),
 
 class Stream:
     def __init__(self, log, name):
-        self.log, self.name = log, name
+        self.log, self.name, self.stream_id = log, name, id(self)
 
     def wait_stream(self, other):
         self.log.append((self.name, "waits for", other.name))
@@ -73,7 +73,7 @@ def program(monkeypatch):
     def set_stream(stream):
         cuda.current = stream
     cuda.set_stream = set_stream
-    torch = types.SimpleNamespace(cuda=cuda, Tensor=Rows, device=lambda *a: a, empty=lambda *a, **k: Rows(cuda.current.name), float32=0, float16=1, bfloat16=2, uint8=3, int32=4)
+    torch = types.SimpleNamespace(cuda=cuda, accelerator=types.SimpleNamespace(current_stream=cuda.current_stream), Tensor=Rows, device=lambda *a: a, empty=lambda *a, **k: Rows(cuda.current.name), float32=0, float16=1, bfloat16=2, uint8=3, int32=4)
     framework = types.SimpleNamespace(Context=Context, RotateSpec=lambda *a: a, LV_F32=0, LV_F16=1, LV_BF16=30, LV_Q8_0=8, LV_Q4_0=2)
     spec = importlib.util.spec_from_file_location("operator_cases", PATH)
     module = importlib.util.module_from_spec(spec)
