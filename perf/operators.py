@@ -375,6 +375,7 @@ class _Framework:
         self.lva = importlib.import_module("llama-vulkan_amd")
         self.ctx = self.lva.Context(device)
         self.stream = torch.cuda.ExternalStream(self.ctx.stream(), device=device)
+        self.stream_id = self.stream.stream_id
         self.work = torch.empty(0, dtype=torch.uint8, device=torch.device("cuda", device))
 
     def workspace(self, size):
@@ -398,9 +399,10 @@ def _type(lva, name):
 
 def _own(s):
     """The calls, in order with the current stream's work: as they are where the program has made the context's stream the current one, by events where it has not."""
-    f, here = _framework(), torch.cuda.current_stream()
-    if here == f.stream:
+    f = _framework()
+    if torch.accelerator.current_stream().stream_id == f.stream_id:
         return _calls(f, s)
+    here = torch.cuda.current_stream()
     f.stream.wait_stream(here)
     with torch.cuda.stream(f.stream):
         out = _calls(f, s)
