@@ -411,7 +411,8 @@ typedef struct {
     const float *sinks;          /* null, or one logit a head that joins the softmax denominator */
 } lv_paged_attn_spec;
 /* out[row][head][dim] = sum_p softmax_p(scale q . k_p) v_p over the positions p that the row's token sees, q and out [tokens][heads][dim] of `type`
- * (LV_F32: as exact as fp32; LV_F16, LV_BF16: products of 16-bit operands, softmax and sums in fp32).  A row that sees nothing is 0.  The rows
+ * (LV_F32: as exact as fp32; LV_F16, LV_BF16: products of 16-bit operands, softmax and sums in fp32).  A row that sees nothing is 0.  A value
+ * that is not finite shows in the rows that see it and in no others, and as itself, whatever its weight (NaN where two disagree).  The rows
  * of keys and values of the new tokens have to be in the cache.  `work`: lv_paged_attention_workspace bytes, null where that is 0. */
 int lv_paged_attention_workspace(lv_ctx *ctx, uint32_t type, const lv_paged_cache *cache, const lv_paged_batch *batch, const lv_paged_attn_spec *spec,
                                  uint64_t *bytes);

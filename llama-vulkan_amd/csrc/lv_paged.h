@@ -306,6 +306,9 @@ __device__ __forceinline__ float pg_apart(float s, float f, float m)
     return x - m;
 }
 
+// what a result x is weighed with: w, but 1 where x is not finite and w has underflowed, 0 times which would be NaN
+__device__ __forceinline__ float pg_weight(float x, float w) { return w == 0.f && x - x != 0.f ? 1.f : w; }
+
 // bits where one of two 16-bit numbers is not finite
 template <bool BF> __device__ __forceinline__ uint32_t pg_special(uint32_t w)
 {
@@ -797,6 +800,12 @@ __global__ __launch_bounds__(256, paged_rows_waves(D, CT, NQ, QT)) void paged_ro
 #pragma unroll
         for (int d = 0; d < DT; d++)
             *reinterpret_cast<float4 *>(res + (wave * 16 + l16) * MERGE + d * 16 + g4 * 4) = make_float4(o[d][i][0] * f, o[d][i][1] * f, o[d][i][2] * f, o[d][i][3] * f);
+        if (CT <= kPgBf16 && special) {
+#pragma unroll
+            for (int d = 0; d < DT; d++)
+#pragma unroll
+                for (int r = 0; r < 4; r++) res[(wave * 16 + l16) * MERGE + d * 16 + g4 * 4 + r] = o[d][i][r] * pg_weight(o[d][i][r], f);
+        }
         __syncthreads();
         for (int u = threadIdx.x; u < 16 * CH; u += 256) {
             const int row = u / CH, c = u % CH * 8;
@@ -834,7 +843,7 @@ __global__ __launch_bounds__(256, paged_rows_waves(D, CT, NQ, QT)) void paged_ro
             }
             f2 = all == 0.f ? 0.f : f2 / all;
 #pragma unroll
-            for (int e = 0; e < 8; e++) y[e] = all == 0.f ? 0.f : y[e] * f2;
+            for (int e = 0; e < 8; e++) y[e] = all == 0.f ? 0.f : y[e] * (CT <= kPgBf16 ? pg_weight(y[e], f2) : f2);
             pg_store8(a.out, a.type, (uint64_t)(it.s.row0 + t2) * a.ldo + (uint64_t)h * D + c, y);
         }
     }
@@ -1058,8 +1067,8 @@ __global__ __launch_bounds__(256, 2) void paged_tile_kernel(PagedAttnArgs a)
     };
     // does some row of the workgroup not see some key of a tile?
     auto partly = [&](uint32_t kb, uint32_t ok) { return kb < all.all_lo || kb + 64 > all.all_hi || ok != 15; };
-    // In such a tile values that no row sees become 0 (0 times what earlier users of a page left there has to be 0), and so do numbers that are not finite, which
-    // are added behind the loop to the rows that see them.
+    // In such a tile values that no row sees become 0 (0 times what earlier users of a page left there has to be 0), and so do numbers that are not finite.  In other
+    // tiles all rows see those, and what they make of a result shows in it.  Behind the loop results are put right where any were found.
     auto clean = [&](uint8_t *vals, uint32_t kb, uint32_t ok) {
         uint32_t odd = 0;
         for (int c = threadIdx.x; c < 64 * CH; c += 256) {
@@ -1225,12 +1234,26 @@ __global__ __launch_bounds__(256, 2) void paged_tile_kernel(PagedAttnArgs a)
             }
         finish();
     }
+    if constexpr (!BLOCKS) {
+        float odd = 0.f;      // NaN where one of the results is not finite
+#pragma unroll
+        for (int d = 0; d < DT; d++)
+#pragma unroll
+            for (int i = 0; i < 16; i++) odd = fmaf(o[d][i], 0.f, odd);
+        if (odd != odd) special = 1;
+    }
     __syncthreads();
-    if (!BLOCKS && special) {
-        // kinds 1 to 3, NaN, inf and -inf: their counts among the keys that a row sees, as a product of ones
+    const bool odd = !BLOCKS && special;
+    if (odd) {
+        // A row that sees numbers that are not finite has their sum, whatever they weigh (a weight of 0 would have made NaN of an infinity).  Kinds 1 to 3, NaN, inf and -inf: their
+        // counts among the keys that a row sees, as a product of ones.
+        pg_f16v sums[DT];
+#pragma unroll
+        for (int d = 0; d < DT; d++)
+#pragma unroll
+            for (int i = 0; i < 16; i++) sums[d][i] = 0.f;
         for (t = t_first; t < t_end; t++) {
             const uint32_t kb = base + t * 64, ok = pages_of(kb);
-            if (!partly(kb, ok)) continue;
             issue(0, page_of(kb + wave * 16), (kb + wave * 16) & (psize - 1));
             asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
             __syncthreads();
@@ -1253,11 +1276,15 @@ __global__ __launch_bounds__(256, 2) void paged_tile_kernel(PagedAttnArgs a)
                         n = pg_mfma32<BF>(pg_only<BF>(values(lds + 64 * ROW, d, j), kind), one, n);
                     }
 #pragma unroll
-                    for (int i = 0; i < 16; i++) o[d][i] += n[i] > 0.f ? add : 0.f;
+                    for (int i = 0; i < 16; i++) sums[d][i] += n[i] > 0.f ? add : 0.f;
                 }
             }
             __syncthreads();
         }
+#pragma unroll
+        for (int d = 0; d < DT; d++)
+#pragma unroll
+            for (int i = 0; i < 16; i++) o[d][i] = sums[d][i] == 0.f ? o[d][i] : sums[d][i];
     }
 
     l += __shfl_xor(l, 32, 64);
@@ -1293,7 +1320,7 @@ __global__ __launch_bounds__(256, 2) void paged_tile_kernel(PagedAttnArgs a)
         for (int i = 0; i < 16; i += 4) {
             float y[4];
 #pragma unroll
-            for (int e = 0; e < 4; e++) y[e] = l == 0.f ? 0.f : o[d][i + e] * f;
+            for (int e = 0; e < 4; e++) y[e] = l == 0.f ? 0.f : o[d][i + e] * (odd ? pg_weight(o[d][i + e], f) : f);
             uint32_t lo2, hi2;
             if (half) {
                 lo2 = pg_bits(y[0], true) | (pg_bits(y[1], true) << 16);
@@ -1345,16 +1372,31 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttnArgs a, float 
         }
         const float big = fmaxf(fmaxf(fmaxf(ms[0], ms[1]), fmaxf(ms[2], ms[3])), top), f = pg_exp2(top - big);
         top = big;
-        all *= f;
-#pragma unroll
-        for (int e = 0; e < V; e++) y[e] *= f;
+        float g[4];
+        bool lost = f == 0.f && all != 0.f;      // has the weight of something underflowed?
 #pragma unroll
         for (int j = 0; j < 4; j++) {
-            const float g = pg_exp2(ms[j] - big);
-            all = fmaf(ls[j], g, all);
-#pragma unroll
-            for (int e = 0; e < V; e++) y[e] = fmaf(v[j][e], g, y[e]);
+            g[j] = pg_exp2(ms[j] - big);
+            lost |= g[j] == 0.f && ls[j] != 0.f;
         }
+        all *= f;
+        if (__any(lost)) {      // care for what is not finite
+#pragma unroll
+            for (int e = 0; e < V; e++) {
+                y[e] *= pg_weight(y[e], f);
+#pragma unroll
+                for (int j = 0; j < 4; j++) y[e] = fmaf(v[j][e], pg_weight(v[j][e], g[j]), y[e]);
+            }
+        } else {
+#pragma unroll
+            for (int e = 0; e < V; e++) {
+                y[e] *= f;
+#pragma unroll
+                for (int j = 0; j < 4; j++) y[e] = fmaf(v[j][e], g[j], y[e]);
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < 4; j++) all = fmaf(ls[j], g[j], all);
     }
 #pragma unroll
     for (int e = 0; e < V; e++)
@@ -1371,14 +1413,26 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttnArgs a, float 
     const float sink = a.sinks ? a.sinks[h] * 1.44269504088896341f : kNothing;
     big = fmaxf(big, sink);
     float total = a.sinks ? pg_exp2(sink - big + lift) : 0.f, z[8];
+    bool lost = false;
 #pragma unroll
     for (int e = 0; e < 8; e++) z[e] = 0.f;
 #pragma unroll
     for (int w = 0; w < WAVES; w++) {
         const float g = pg_exp2(tops[first + w][0] - big);
+        lost |= g == 0.f && tops[first + w][1] != 0.f;
         total = fmaf(tops[first + w][1], g, total);
 #pragma unroll
         for (int e = 0; e < 8; e++) z[e] = fmaf(sums[first + w][lane * 8 + e], g, z[e]);
+    }
+    if (lost) {      // once more, with care for what is not finite
+#pragma unroll
+        for (int e = 0; e < 8; e++) z[e] = 0.f;
+#pragma unroll 1
+        for (int w = 0; w < WAVES; w++) {
+            const float g = pg_exp2(tops[first + w][0] - big);
+#pragma unroll
+            for (int e = 0; e < 8; e++) z[e] = fmaf(sums[first + w][lane * 8 + e], pg_weight(sums[first + w][lane * 8 + e], g), z[e]);
+        }
     }
     const float f = 1.f / total;
 #pragma unroll

@@ -366,6 +366,34 @@ def test_attention_of_numbers_that_are_not_finite_in_chunks(dev, cache, kind, di
     assert np.isfinite(want[:30]).all() and np.isinf(want[30]).any() and np.isnan(want[75:80]).any()
 
 
+@pytest.mark.parametrize("sinks", [False, True])
+@pytest.mark.parametrize("cache,kind", [(F16, F16), (F16, BF16), (BF16, BF16), (F16, F32), (BF16, F32)], ids=lambda k: ref.NAMES[k])
+@pytest.mark.parametrize("dim,new", [(64, 90), (128, 90), (64, 2), (128, 2), (32, 90)])
+@pytest.mark.parametrize("keys", [330, 1100])      # one launch; cut into parts that a second one puts together
+def test_attention_of_values_that_are_not_finite_and_weigh_next_to_nothing(dev, cache, kind, dim, new, keys, sinks):
+    """An infinity times a weight is infinite, however small the weight is: it shows as itself in every row that sees it.  The first keys' scores are 200 below the others' (weights of
+    e^-200, which 64 bits hold and 32 do not), some of the later ones' 25 (2^-36: 0 as fp16); with a learned logit 300 above all of them every weight is e^-300 or less."""
+    rng = np.random.default_rng(63)
+    pool = ref.Pool(cache, 1, dim, 16, keys // 16 + 3, rng)
+    step = ref.Step(pool, [keys], [new], rng)
+    unit = 8.0 / dim                      # of a key: a score of 1 with queries of 1 and a scale of 0.125
+    far, some = 140, (150, 177, 200, 233)
+    for p in range(keys):
+        at = step.place(pool, 0, p)
+        pool.put(at[0], 0, 0, at[1], np.full(dim, unit * (-200 if p < far else -25 if p in some else 0)) + rng.standard_normal(dim) * 0.01)
+        v = rng.standard_normal(dim)
+        for d, x in {7: {0: np.inf}, 100: {0: np.inf, 1: -np.inf, 2: np.inf}, 139: {3: -np.inf, 4: np.nan}, 150: {5: np.inf, 6: -np.inf}, 200: {6: np.inf}, 233: {2: -np.inf, 7: np.nan}}.get(p, {}).items():
+            v[d] = x
+        pool.put(at[0], 0, 1, at[1], v)
+    s = np.array([300, 0], dtype=np.float32) if sinks else None
+    got, held = run_attention(dev, pool, step, np.ones((new, 2, dim)), kind, 2, 0.125, 0, 0, s)
+    want, size, reach, seen, mass = ref.attention(pool, step, held, 2, 0.125, 0, 0, s)
+    assert np.isposinf(want[..., [0, 5]]).all() and np.isneginf(want[..., [1, 3]]).all() and np.isnan(want[..., [2, 4, 6, 7]]).all() and np.isfinite(want[..., 8:]).all()
+    assert np.array_equal(got[..., :8], want[..., :8], equal_nan=True)
+    bound = ref.attention_bound(want[..., 8:], size[..., 8:], reach, seen, mass[..., 8:], dim, kind, cache)
+    assert np.all(np.abs(got[..., 8:] - want[..., 8:]) <= bound)
+
+
 @pytest.mark.parametrize("dim", [64, 128])
 @pytest.mark.parametrize("cache,kind,window", [(F16, F16, 0), (BF16, BF16, 0), (F16, BF16, 700), (Q8, F16, 0)], ids=str)
 def test_attention_of_a_chunk_behind_a_long_context(dev, cache, kind, window, dim):
