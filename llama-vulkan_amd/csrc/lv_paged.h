@@ -880,10 +880,10 @@ template <int N> __device__ __forceinline__ void pg_load_direct(uint32_t to, con
     if constexpr (N == 4)
         asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %5\n\tglobal_load_lds_dwordx4 %2, %5 offset:1024\n\t"
                      "global_load_lds_dwordx4 %3, %5 offset:2048\n\tglobal_load_lds_dwordx4 %4, %5 offset:0xc00"
-                     : : "s"(__builtin_amdgcn_readfirstlane(to)), "v"(at[0]), "v"(at[1]), "v"(at[2]), "v"(at[3]), "s"(base) : "memory");
+                     : : "s"(__builtin_amdgcn_readfirstlane(to)), "v"(at[0]), "v"(at[1]), "v"(at[2]), "v"(at[3]), "s"(base) : "memory", "m0");
     else
         asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %3\n\tglobal_load_lds_dwordx4 %2, %3 offset:1024"
-                     : : "s"(__builtin_amdgcn_readfirstlane(to)), "v"(at[0]), "v"(at[1]), "s"(base) : "memory");
+                     : : "s"(__builtin_amdgcn_readfirstlane(to)), "v"(at[0]), "v"(at[1]), "s"(base) : "memory", "m0");
 }
 
 constexpr int kPagedTileRows = 128;

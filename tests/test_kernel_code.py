@@ -100,3 +100,16 @@ def test_nothing_moves_between_matrix_products_of_tiles_with_units(code_objects)
                         inside, halves = False, halves + 1
             assert not inside and halves == 2 * (5 if "ELi80E" in name else 6), (name, halves)
     assert seen == 6      # three epilogues of each
+
+
+def test_inline_assembly_names_what_it_writes():
+    """m0 is written for direct loads: a value that the compiler kept there would be lost if the statement did not say so"""
+    csrc = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "llama-vulkan_amd", "csrc")
+    writes = 0
+    for f in sorted(os.listdir(csrc)):
+        text = open(os.path.join(csrc, f)).read()
+        for statement in re.findall(r"\basm\b[^;]*?\((?:[^\"()]|\"(?:[^\"\\]|\\.)*\"|\((?:[^()]|\([^()]*\))*\))*\)\s*;", text):
+            if re.search(r"\bs_\w+ m0\b", statement):
+                writes += 1
+                assert re.search(r":[^:]*\"m0\"[^:]*\)\s*;$", statement), (f, statement)
+    assert writes >= 2
