@@ -321,6 +321,36 @@ def test_attention_of_hundreds_of_sequences(dev, columns):
     check_attention(dev, rng, F16, F16, 2, 1, 64, 16, lens.tolist(), new.tolist(), pad=2)
 
 
+@pytest.mark.parametrize("cache,kind", [(F16, F16), (Q8, BF16), (BF16, F32)], ids=lambda k: ref.NAMES[k])
+@pytest.mark.parametrize("seqs,heads,kv_heads,long,longest", [
+    (100, 2, 1, (5, 70, 99), 1500),        # fewer sequences than compute units, few rows: the join has four waves a row
+    (100, 12, 1, (5, 63, 64, 99), 1500),   # and one wave a row
+    (150, 4, 2, (0, 64, 149), 3000),       # as many sequences' key heads as compute units: cut for evenness
+    (300, 2, 2, (5, 130, 299), 5000),      # twice as many, and in longer parts
+], ids=str)
+def test_attention_of_more_sequences_than_a_wave_looks_at_that_are_cut(dev, cache, kind, seqs, heads, kv_heads, long, longest):
+    """64 sequences are looked at at a time: what those before them take is carried on, in the launch and in the join"""
+    lva, ctx = dev.lva, dev.ctx
+    rng = np.random.default_rng(64)
+    lens = rng.integers(1, 40, seqs)
+    lens[list(long)] = [longest - 61 * i for i in range(len(long))]
+    new = np.minimum(rng.integers(0, 3, seqs), lens)
+    new[list(long)] = (1, 2, 1, 1)[:len(long)]
+    new[1::7] = 1
+    seen = {}
+
+    def edit(pool, step):      # the call once more by itself: what has been cut is in the workspace
+        seen["q"] = ref.encode(rng.standard_normal((step.tokens, heads * 64)), kind)
+        _, c = dev.cache(pool)
+        b, spec = dev.batch(step), lva.PagedAttnSpec(heads, 0.125, 0, 0, None)
+        n = ctx.paged_attention_workspace(kind, c, b, spec)
+        assert n > 0
+        work, out = dev.put(np.full(n, 0xFF, np.uint8)), dev.put(np.zeros_like(seen["q"]))
+        ctx.paged_attention(out, heads * 64, dev.put(seen["q"]), heads * 64, kind, c, b, spec, work, n)
+        assert np.count_nonzero(dev.get(work, (n // 4,), np.uint32) != 0xFFFFFFFF) >= 2 * 2 * len(long) * kv_heads      # maxima and sums of two parts of each at least
+    check_attention(dev, rng, cache, kind, heads, kv_heads, 64, 16, lens.tolist(), new.tolist(), pad=2, sinks=True, edit=edit)
+
+
 @pytest.mark.parametrize("cache", [F16, BF16, Q8, Q4], **KINDS)
 def test_attention_of_large_scores(dev, cache):
     """one key takes nearly all weight: 2^-100 and less for the others"""
@@ -623,6 +653,25 @@ def test_verify(dev, seqs, drafts, vocab, sampled):
         assert np.array_equal(got[1], want[1]) and np.array_equal(got[0], want[0])
 
 
+@pytest.mark.parametrize("vocab", [500, 40000])      # one launch, two
+@pytest.mark.parametrize("drafts", [63, 64])
+def test_verify_drafts_that_all_stand(dev, drafts, vocab):
+    """as many drafts as a wave has lanes, none of them refused: the next token is from the row behind them"""
+    rng = np.random.default_rng(65)
+    target = probabilities(rng, (2, drafts + 1, vocab))
+    draft = target[:, :drafts].copy()
+    tokens = np.array([[rng.choice(vocab, p=r.astype(np.float64) / r.astype(np.float64).sum()) for r in s] for s in draft])
+    uniforms = np.minimum(rng.random((2, drafts + 1)).astype(np.float32), np.float32(0.99999))
+    draft[1, drafts - 1] = 0              # the second sequence's last one is one that the draft never gives: it stands too
+    got = run_verify(dev, target, draft, tokens, None, uniforms)
+    want = ref.verify(target, draft, tokens, np.full(2, drafts), uniforms)
+    assert np.all(want[1] == drafts) and np.array_equal(got[1], want[1]) and np.array_equal(got[0], want[0])
+    target[0, drafts - 1, int(tokens[0, drafts - 1])] = 0      # the very last one refused
+    got = run_verify(dev, target, draft, tokens, None, uniforms)
+    want = ref.verify(target, draft, tokens, np.full(2, drafts), uniforms)
+    assert want[1].tolist() == [drafts - 1, drafts] and np.array_equal(got[1], want[1]) and np.array_equal(got[0], want[0])
+
+
 def test_verify_borders(dev):
     """random numbers at their ends, weights of 0 at a row's ends and in its middle, rows without weight, drafts outside the vocabulary, NaN"""
     rng = np.random.default_rng(52)
@@ -796,6 +845,29 @@ def test_a_step_of_drafts_captured_and_replayed(dev, cache, kind, columns):
         lva.check(ctx.lib.lv_dev_zero(ctx.h, other, 1 << 20))      # other work between the replays
         lens = lens - (drafts - acc.astype(np.int64))              # refused drafts' rows are written over by the next step
     graph.close()
+
+
+@pytest.mark.parametrize("cache,kind", [(F16, F32), (BF16, BF16), (Q8, BF16), (Q4, F16)], ids=lambda k: ref.NAMES[k])
+@pytest.mark.parametrize("lens,new", [([1500, 400, 90], [1, 3, 1]), ([1500, 400], [200, 70]), ([300], [300])], ids=str)
+def test_calls_repeat_themselves(dev, cache, kind, lens, new):
+    """the same call ten times, other work between: the same bits"""
+    lva, ctx = dev.lva, dev.ctx
+    rng = np.random.default_rng(66)
+    pool = ref.Pool(cache, 2, 128, 16, 140, rng)
+    pool.bytes[:] = rng.integers(0, 48, pool.bytes.shape, dtype=np.uint8)      # small finite numbers and scales
+    step = ref.Step(pool, lens, new, rng)
+    _, c = dev.cache(pool)
+    b, spec = dev.batch(step), lva.PagedAttnSpec(8, 0.01, 0, 0, None)
+    q = dev.put(ref.encode(rng.standard_normal((step.tokens, 1024)), kind))
+    n = ctx.paged_attention_workspace(kind, c, b, spec)
+    work, out = dev.put(np.full(n + 16, 0xFF, np.uint8)), dev.put(np.zeros((step.tokens, 1024), ref.DTYPE[kind]))
+    first = None
+    for turn in range(10):
+        lva.check(ctx.lib.lv_dev_zero(ctx.h, out, step.tokens * 1024 * ref.BYTES[kind]))
+        ctx.paged_attention(out, 1024, q, 1024, kind, c, b, spec, work, n)
+        got = dev.get(out, (step.tokens, 1024 * ref.BYTES[kind]), np.uint8)
+        first = got if first is None else first
+        assert first.any() and np.array_equal(got, first), turn
 
 
 def test_two_contexts_at_once(lva, ctx, dev):

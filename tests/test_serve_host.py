@@ -266,6 +266,19 @@ def test_layout(ask, kind, dim, page):
     assert codes == ((1 << 20) * 64 - 1) * pool.block + pool.half + (page - 1) * pool.code_row
 
 
+@pytest.mark.parametrize("dim,page", [(32, 16), (32, 1024), (64, 16), (256, 16)])
+def test_layout_of_the_shortest_rows(ask, dim, page):
+    """4 bits: a row of codes is as short as the alignment that loads rest on"""
+    pool = ref.Pool(ref.Q4, 3, dim, page, 4)
+    for p, h, w, t in [(p, h, w, t) for p in (0, 3) for h in (0, 2) for w in (0, 1) for t in (0, 1, page - 1)]:
+        (codes, scales, block), = ask([("row", ref.Q4, 3, dim, page, 4, p, h, w, t)])
+        c, s = pool.row(p, h, w, t)
+        base = pool.bytes.ctypes.data
+        assert block == pool.block
+        assert codes == c.ctypes.data - base and codes % 16 == 0
+        assert scales == s.ctypes.data - base and scales % 2 == 0
+
+
 def test_pages_that_are_not_there(ask):
     row = [2, 9, 10, 0xFFFFFFFF, 0]
     q = [("page", 16, 10, p, len(row), *row) for p in (0, 15, 16, 31, 32, 48, 64, 79, 80, 1 << 30, 0xFFFFFFFF)]
