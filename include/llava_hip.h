@@ -370,7 +370,7 @@ int lv_ctx_stream(const lv_ctx *ctx, void **stream);
  * its low nibble and j + 16 in its high one, minus 8; both with an fp16 scale for every 32 elements (the blocks of GGML files, codes and scales apart).
  * A block is stored with the scale d = fp16(min(max|x| * (1 / 127), 515.5)) and codes rint(x * (1 / d)) in -127 .. 127 (LV_Q8_0), or with
  * d = fp16(clamp(m * -0.125, -8188, 8188)), m the element furthest from 0 (the positive one of two), and codes in -8 .. 7 (LV_Q4_0); steps in fp32, ties to
- * even; a scale of 0 is +0, and so are its codes.  No stored value is beyond 65504; a NaN is stored as 0. */
+ * even; a scale of 0 is +0, and so are its codes.  No stored value is beyond 65504; a NaN is stored as 0.  What else a program puts into a pool has finite scales. */
 typedef struct {
     void *data;
     uint32_t type;               /* LV_F16, LV_BF16, LV_Q8_0, LV_Q4_0 */
@@ -383,7 +383,7 @@ int lv_paged_cache_bytes(const lv_paged_cache *cache, uint64_t *bytes);
 
 /* The new tokens of a step.  Rows starts[b] .. starts[b + 1] - 1 of a call's tensors belong to sequence b and are the last of its lens[b]
  * tokens; a sequence may have none.  Position i of sequence b lies in page table[b * table_ld + i / page].  Rows from starts[seqs] on belong to nobody and
- * are left as they were (a padded batch).  starts are non-decreasing and at most `tokens`.  A position whose page is not in 0 .. pages - 1, or beyond
+ * are left as they were (a padded batch).  starts are non-decreasing and at most `tokens`; a length of more than 2^30 counts as 2^30.  A position whose page is not in 0 .. pages - 1, or beyond
  * the table, is never touched: it is not written, not read back, and hidden from attention; so is a position before 0 (lens[b] less than the new
  * tokens). */
 typedef struct {
@@ -438,8 +438,8 @@ int lv_kernel_rotate(lv_ctx *ctx, void *out, uint32_t ldo, const void *x, uint32
 /* Which drafted tokens stand.  Of sequence b, draft i (0 <= i < counts[b]) with token x stands while uniforms[b][i] * draft[b][i][x] < target[b][i][x] and
  * all before it stand.  The next token comes from the row r = number of those that stand: from max(0, target[b][r] - draft[b][r]) if draft r was
  * refused, from target[b][r] if there was none; it is the first j whose running sum is more than uniforms[b][drafts] times the whole.  Where no weight is left,
- * the draw is from target[b][r], and where that has none either, it is token 0.  Weights that are negative or NaN count as 0, a draft outside the vocabulary
- * is refused.  draft null: the drafts were picked, not sampled; their probability is 1.  Products and sums in double. */
+ * the draw is from target[b][r], and where that has none either, it is token 0.  A weight, the difference or the target itself, that is negative or NaN counts as 0, a
+ * comparison with NaN does not hold, a draft outside the vocabulary is refused.  draft null: the drafts were picked, not sampled; their probability is 1.  Products and sums in double. */
 typedef struct {
     uint32_t seqs, drafts, vocab;    /* drafts: columns of `tokens`, 1 to 64 */
     const float *target;             /* [seqs][drafts + 1][vocab] probabilities, ld_target floats a row */

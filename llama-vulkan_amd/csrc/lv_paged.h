@@ -346,14 +346,14 @@ __device__ __forceinline__ pg_s4 pg_read_columns(const uint8_t *p)
 // 32-bit queries they enter as two fp16 pieces, which hold them exactly: 19 bits at most, the last of them 2^-24 or more, as the scale's is.
 // FINE: rows of codes and an fp16 result.  Its own rounding is no coarser than the weights' and the scaled values' are, and with both the error is 1.6 times the result's
 // rounding alone; the weights enter as two pieces, and it is 1.4 times (single tokens and drafts: 1 to 7 % of the time).  Beside a bf16 result neither shows.
-typedef uint32_t pg_u2 __attribute__((ext_vector_type(2)));
 template <int BYTES> struct PgWord { typedef uint32_t type; };
 template <> struct PgWord<8> { typedef pg_u2 type; };
-// waves a SIMD that the registers are cut for: as many as leave none in memory
+// waves a SIMD that the registers are cut for: as many as leave none in memory, but two where 32 rows of 32-bit queries over fp16 rows (27 registers in memory) or rows of
+// 8 bits (17) have heads of 128
 constexpr int paged_rows_waves(int D, int CT, int NQ, int QT)
 {
     if (D == 256) return 1;
-    if (D == 128 && QT == 2 && NQ == 3) return 1;      // 59 registers in memory cost more than a second wave gains (1024 tokens, the last of 4096: 340 us and 281)
+    if (D == 128 && QT == 2 && NQ == 3) return 1;      // here 59 registers in memory cost more than a second wave gains (1024 tokens, the last of 4096: 340 us and 281)
     if (D == 128) return QT == 1 && NQ == 1 && CT >= kPgQ8 ? 3 : 2;
     return NQ > 1 && QT == 2 ? 2 : 3;
 }
@@ -858,7 +858,8 @@ __global__ __launch_bounds__(256, paged_rows_waves(D, CT, NQ, QT)) void paged_ro
 // The running maximum is a reference: weights are formed with it at once, and only where their sum says that a score is far above it are the maximum taken, the results
 // rescaled and the weights formed anew.  Most tiles do without the maximum's 48 vector instructions (half of them make numbers canonical).
 // Weights enter the second product as one fp16 (2^-11) or bf16 (2^-8) number: beside a 16-bit result's own rounding, over all the keys of a row.
-// FINE: as two fp16 pieces, as above (1024 tokens, the last of 4096, 8 bits: 128 and 165 us; 4 bits 125 and 157).  Rows of codes come through registers instead of direct loads.
+// FINE: as two fp16 pieces, as above (1024 tokens, the last of 4096, 8 bits: 119 and 154 us; 4 bits 118 and 149).  Rows of codes come through registers instead of direct loads,
+// some of which are in memory with heads of 128: 3 with 8 bits, 16 and 8 with 8 and 4 bits and FINE.
 typedef float pg_f16v __attribute__((ext_vector_type(16)));
 
 

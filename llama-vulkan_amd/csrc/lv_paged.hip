@@ -17,7 +17,8 @@ struct AttnPlan {
 
 // Workgroups a compute unit that share the work of a call (lv_paged_plan.h)
 constexpr uint32_t kTargetPerUnit = 2;
-// The kernel for tiles takes sequences of more rows than these in the mean (rows of a sequence and key head: new tokens times the heads that share it).  us, rows kernel and
+// The kernel for tiles takes calls whose sequences have more rows than these in the mean, one kernel for all of them: in the mean of all rows of the tensors, those behind the last
+// sequence too, over all sequences, those without new tokens too, since the host knows no others (rows of a sequence and key head: new tokens times the heads that share it).  us, rows kernel and
 // tiles, 16 sequences of 3000 keys, 8 key heads of 128: fp16 32 rows 39 40, 40 rows 45 41, 64 rows 47 44, 128 rows 65 51; 8 bits 40 rows 50 52, 64 rows 51 55, 80 rows 79 58
 constexpr uint32_t kTileRows = 32, kTileRowsBlocks = 64;
 // Rows from which the second launch has a wave for each instead of four.
